@@ -56,6 +56,32 @@ LAYER_EXPORTS = (
     "sfa_moe_ffn",
 )
 
+# include/sfa_window.h (windowed models' attention node; also in libsfa.so)
+WINDOW_EXPORTS = (
+    "sfa_rope_desc_check",
+    "sfa_norm_rope_kv_append",
+    "sfa_decode_window_workspace_bytes",
+    "sfa_attn_decode_window",
+    "sfa_prefill_window_workspace_bytes",
+    "sfa_attn_prefill_window",
+)
+
+SFA_ROPE_NORMAL = 0
+SFA_ROPE_NEOX = 2
+SFA_AXES_BLOCKS = 0
+SFA_AXES_INTERLEAVED = 1
+
+
+class SfaRopeDesc(ctypes.Structure):
+    _fields_ = [
+        ("n_rot", ctypes.c_int32),
+        ("pairing", ctypes.c_int32),
+        ("freq_base", ctypes.c_float),
+        ("n_axis", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("layout", ctypes.c_int32),
+    ]
+
 
 class SfaKvDesc(ctypes.Structure):
     _fields_ = [
@@ -149,6 +175,21 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     lib.sfa_moe_workspace_bytes.restype = ctypes.c_size_t
     lib.sfa_moe_ffn.argtypes = [P, P, P, P, P, P, P, i32, i32, i32, i32, i32, i32, P, ctypes.c_size_t, P, P]
     lib.sfa_moe_ffn.restype = ctypes.c_int
+    # windowed models' attention node (include/sfa_window.h)
+    f32, i64, size = ctypes.c_float, ctypes.c_int64, ctypes.c_size_t
+    R = ctypes.POINTER(SfaRopeDesc)
+    lib.sfa_rope_desc_check.argtypes = [R, i32]
+    lib.sfa_rope_desc_check.restype = ctypes.c_int
+    lib.sfa_norm_rope_kv_append.argtypes = [D, R, P, i64, P, P, i64, P, i64, P, P, f32, P, P, P, i32, P, i32, P]
+    lib.sfa_norm_rope_kv_append.restype = ctypes.c_int
+    lib.sfa_decode_window_workspace_bytes.argtypes = [D, i32, i32, i32, i32]
+    lib.sfa_decode_window_workspace_bytes.restype = size
+    lib.sfa_attn_decode_window.argtypes = [D, P, P, P, i32, P, i32, i32, i32, i32, f32, P, size, P]
+    lib.sfa_attn_decode_window.restype = ctypes.c_int
+    lib.sfa_prefill_window_workspace_bytes.argtypes = [D, i32, i32, i32, i32]
+    lib.sfa_prefill_window_workspace_bytes.restype = size
+    lib.sfa_attn_prefill_window.argtypes = [D, P, P, P, i32, i32, i32, i32, i32, f32, P, size, P]
+    lib.sfa_attn_prefill_window.restype = ctypes.c_int
     _lib = lib
     return lib
 

@@ -9,15 +9,17 @@ tensors, so a call does no host-to-device copy.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
 import torch
 
 from . import _lib
-from ._lib import SFA_KV_F16, SFA_KV_F32, SFA_KV_Q8_0, SfaKvDesc
+from ._lib import (SFA_AXES_BLOCKS, SFA_AXES_INTERLEAVED, SFA_KV_F16, SFA_KV_F32, SFA_KV_Q8_0, SFA_ROPE_NEOX,
+                   SFA_ROPE_NORMAL, SfaKvDesc, SfaRopeDesc)
 
-__all__ = ["PagedKV", "row_bytes", "SFA_KV_F32", "SFA_KV_F16", "SFA_KV_Q8_0"]
+__all__ = ["PagedKV", "row_bytes", "rope_desc", "SFA_KV_F32", "SFA_KV_F16", "SFA_KV_Q8_0"]
 
 
 def row_bytes(kv_type: int, head_dim: int) -> int:
@@ -30,6 +32,26 @@ def row_bytes(kv_type: int, head_dim: int) -> int:
     raise ValueError(f"unsupported kv type {kv_type}")
 
 
+def rope_desc(head_dim: int, freq_base: float, n_rot: int | None = None, neox: bool = False,
+              sections=None, interleaved: bool = False) -> SfaRopeDesc:
+    """The rotation of ``norm_rope_append``: the first n_rot elements of a head
+    (all by default) in pairs (x[2i], x[2i+1]), or (x[i], x[i + n_rot/2]) with
+    ``neox``; ``sections``: the pairs of each axis of a position, in blocks or
+    dealt in turn (``interleaved``)."""
+    d = SfaRopeDesc()
+    d.n_rot = head_dim if n_rot is None else n_rot
+    d.pairing = SFA_ROPE_NEOX if neox else SFA_ROPE_NORMAL
+    d.freq_base = freq_base
+    sections = [d.n_rot // 2] if sections is None else list(sections)
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("a position has one to four axes")
+    d.n_axis = len(sections)
+    d.sections[:len(sections)] = sections
+    d.layout = SFA_AXES_INTERLEAVED if interleaved else SFA_AXES_BLOCKS
+    _lib.check(_lib.load().sfa_rope_desc_check(ctypes.byref(d), head_dim), "rope descriptor")
+    return d
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -38,6 +60,23 @@ def _stream(stream) -> int:
     if stream is None:
         return _lib.current_stream()
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _on(device: torch.device):
+    """The device current for a call, where it is another one."""
+    if device.index in (None, torch.cuda.current_device()):
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _empty(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """An uninitialised tensor in the allocator's order of the stream that uses
+    it: freed while the call still runs, it is handed on to that stream alone."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(_stream(stream), device)
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 class PagedKV:
@@ -53,6 +92,7 @@ class PagedKV:
         self.page_bytes = row_bytes(kv_type, head_dim) * n_head_kv * page_size
         self.k = torch.zeros((n_layer, n_pages, self.page_bytes), dtype=torch.uint8, device=self.device)
         self.v = torch.zeros_like(self.k)
+        self._dev = self.k.device  # with its index
         if n_cold_pages:
             # host-pinned cold pool, readable by the GPU over the host link
             self.k_cold = torch.zeros((n_layer, n_cold_pages, self.page_bytes), dtype=torch.uint8,
@@ -221,4 +261,103 @@ class PagedKV:
                                         int(q_pos0), T, int(kv_lo),
                                         float(scale if scale is not None else self.scale),
                                         _stream(stream)), "sfa_attn_prefill")
+        return out
+
+    # -- windowed models: head norms and rotations on the append, window + sinks ----
+    def _is(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple | None = None) -> torch.Tensor:
+        if t.dtype is not dtype or t.device != self._dev or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {dtype} tensor on {self._dev}")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"{what} has shape {tuple(t.shape)}, not {shape}")
+        return t
+
+    def _heads(self, t: torch.Tensor, what: str, n_tok: int, heads: int) -> int:
+        """Checks [n_tok, heads, hd] f32 rows, whole within a token; the stride between tokens."""
+        if t.dtype is not torch.float32 or t.device != self._dev or t.shape != (n_tok, heads, self.head_dim):
+            raise ValueError(f"{what} must be float32 [{n_tok}, {heads}, {self.head_dim}] on {self._dev}")
+        step, head, one = t.stride()
+        if one != 1 or (heads > 1 and head != self.head_dim):
+            raise ValueError(f"{what}: the heads of a token must lie one after the other")
+        return step
+
+    def norm_rope_append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                         seq: torch.Tensor, pos: torch.Tensor, page_table: torch.Tensor, rope: SfaRopeDesc,
+                         q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                         eps: float = 1e-6, rope_pos: torch.Tensor | None = None,
+                         q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
+        """Norms the heads of Q and K (q_norm, k_norm [hd], each optional),
+        rotates them by ``rope`` and appends K and V; returns the rotated Q
+        [n_tok, Hq, hd] (``q_out``, which may be a contiguous q itself).
+        q [n_tok, Hq, hd] (or None), k, v [n_tok, Hkv, hd] f32 may be slices of
+        the stacked Q/K/V rows; rope_pos [n_axis, n_tok] int32 (default: pos on
+        every axis)."""
+        n_tok = seq.numel()
+        ks = self._heads(k, "k", n_tok, self.n_head_kv)
+        vs = self._heads(v, "v", n_tok, self.n_head_kv)
+        self._is(seq, "seq", torch.int32)
+        self._is(pos, "pos", torch.int32, seq.shape)
+        self._is(page_table, "page_table", torch.int32)
+        qs = 0
+        if q is not None:
+            qs = self._heads(q, "q", n_tok, self.n_head)
+            if q_out is None:
+                q_out = _empty((n_tok, self.n_head, self.head_dim), torch.float32, self._dev, stream)
+            else:
+                self._is(q_out, "q_out", torch.float32, (n_tok, self.n_head, self.head_dim))
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None:
+                self._is(w, what, torch.float32, (self.head_dim,))
+        if rope_pos is not None:
+            self._is(rope_pos, "rope_pos", torch.int32, (rope.n_axis, n_tok))
+        with _on(self._dev):
+            _lib.check(_lib.load().sfa_norm_rope_kv_append(
+                self._descs[layer], rope, _ptr(q), qs, _ptr(q_out), k.data_ptr(), ks, v.data_ptr(), vs, _ptr(q_norm),
+                _ptr(k_norm), eps, seq.data_ptr(), pos.data_ptr(), _ptr(rope_pos), n_tok, page_table.data_ptr(),
+                page_table.shape[-1], _stream(stream)), "sfa_norm_rope_kv_append")
+        return q_out
+
+    def decode_window(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, seq_len: torch.Tensor,
+                      max_seq_len: int, window: int, n_sink: int = 0, out: torch.Tensor | None = None,
+                      scale: float | None = None, stream=None) -> torch.Tensor:
+        """q [B, Hq, hd] f32 -> out [B, Hq*hd] f32: the token at seq_len[b] - 1
+        attends the last ``window`` positions and the first ``n_sink``.  The
+        workspace is the call's own."""
+        B = seq_len.numel()
+        self._is(q, "q", torch.float32, (B, self.n_head, self.head_dim))
+        self._is(seq_len, "seq_len", torch.int32)
+        self._is(page_table, "page_table", torch.int32, (B, page_table.shape[-1]))
+        shape = (B, self.n_head * self.head_dim)
+        out = _empty(shape, torch.float32, self._dev, stream) if out is None else self._is(out, "out", torch.float32, shape)
+        lib = _lib.load()
+        d = self._descs[layer]
+        with _on(self._dev):
+            ws = _empty((lib.sfa_decode_window_workspace_bytes(d, B, max_seq_len, window, n_sink),), torch.uint8,
+                        self._dev, stream)
+            _lib.check(lib.sfa_attn_decode_window(
+                d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.shape[1], seq_len.data_ptr(), window,
+                n_sink, B, max_seq_len, self.scale if scale is None else scale, ws.data_ptr(), ws.numel(),
+                _stream(stream)), "sfa_attn_decode_window")
+        return out
+
+    def prefill_window(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, q_pos0: int, window: int,
+                       n_sink: int = 0, out: torch.Tensor | None = None, scale: float | None = None,
+                       stream=None) -> torch.Tensor:
+        """q [T, Hq, hd] f32 of one sequence -> out [T, Hq*hd] f32: the token at
+        position t attends the ``window`` positions up to t and the first
+        ``n_sink``.  The workspace is the call's own."""
+        T = q.shape[0]
+        self._is(q, "q", torch.float32, (T, self.n_head, self.head_dim))
+        self._is(page_table, "page_table", torch.int32, (page_table.numel(),))
+        shape = (T, self.n_head * self.head_dim)
+        out = _empty(shape, torch.float32, self._dev, stream) if out is None else self._is(out, "out", torch.float32, shape)
+        lib = _lib.load()
+        d = self._descs[layer]
+        with _on(self._dev):
+            need = lib.sfa_prefill_window_workspace_bytes(d, q_pos0, T, window, n_sink)
+            ws = _empty((need,), torch.uint8, self._dev, stream) if need else None
+            _lib.check(lib.sfa_attn_prefill_window(
+                d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.numel(), q_pos0, T, window, n_sink,
+                self.scale if scale is None else scale, _ptr(ws), need, _stream(stream)), "sfa_attn_prefill_window")
         return out

@@ -1,0 +1,121 @@
+"""The windowed attention node's C ABI: what the library exports and what it refuses, on the host."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from strataflow_amd import _lib
+from strataflow_amd.paged_kv import rope_desc
+
+from .test_abi import INCLUDE, declared_symbols, desc
+
+OK, BAD, UNS = _lib.SFA_OK, _lib.SFA_ERR_INVALID_ARGUMENT, _lib.SFA_ERR_UNSUPPORTED
+P = 0x1000  # never dereferenced
+MAX = 2**31 - 1
+
+
+def test_header_matches_binding_list():
+    names = declared_symbols(INCLUDE / "sfa_window.h")
+    assert names == set(_lib.WINDOW_EXPORTS)
+    lib = _lib.load()
+    for name in names:
+        assert hasattr(lib, name), name
+
+
+def append(kv=None, rope=None, **kw):
+    a = dict(q=P, qs=32 * 128, out=2 * P, k=P, ks=8 * 128, v=P, vs=8 * 128, qn=P, kn=P, eps=1e-6, seq=P, pos=P, rp=None, n=2,
+             table=P, mp=4)
+    a.update(kw)
+    return _lib.load().sfa_norm_rope_kv_append(kv or desc(), rope or rope_desc(128, 1e4), a["q"], a["qs"], a["out"], a["k"], a["ks"],
+                                               a["v"], a["vs"], a["qn"], a["kn"], a["eps"], a["seq"], a["pos"], a["rp"], a["n"],
+                                               a["table"], a["mp"], None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(n=0), OK), (dict(n=-1), BAD), (dict(mp=0), BAD), (dict(eps=-1.0), BAD), (dict(eps=float("nan")), BAD),
+    (dict(k=None), BAD), (dict(v=None), BAD), (dict(seq=None), BAD), (dict(pos=None), BAD), (dict(table=None), BAD),
+    (dict(q=None), BAD), (dict(out=None), BAD),               # q without q_out and the other way round
+    (dict(qs=32 * 128 - 4), BAD), (dict(ks=8 * 128 - 4), BAD), (dict(vs=0), BAD),
+    (dict(qs=32 * 128 + 2), UNS), (dict(ks=8 * 128 + 1), UNS), (dict(vs=8 * 128 + 3), UNS),
+    (dict(out=P, qs=48 * 128), BAD),                            # in place on rows with a stride
+    (dict(q=P + 4), UNS), (dict(out=P + 8), UNS), (dict(k=P + 4), UNS), (dict(v=P + 4), UNS),
+])
+def test_append_refusals(kw, want):
+    assert append(**kw) == want
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(n_rot=0), BAD), (dict(n_rot=136), BAD), (dict(n_rot=12), UNS), (dict(pairing=1), BAD), (dict(freq_base=0.0), BAD),
+    (dict(freq_base=float("inf")), BAD), (dict(freq_base=float("nan")), BAD), (dict(n_axis=0), BAD), (dict(n_axis=5), BAD),
+    (dict(n_axis=3, sections=(20, 20, 20)), BAD), (dict(n_axis=2, sections=(-1, 65)), BAD), (dict(n_axis=2, sections=(32, 32), layout=7), BAD),
+    (dict(n_axis=2, sections=(31, 33), layout=1), BAD),         # 33 pairs of axis 1 are not there to be dealt
+    (dict(n_axis=2, sections=(32, 32), layout=1), OK), (dict(n_axis=3, sections=(0, 64, 0)), OK), (dict(n_rot=8), OK),
+])
+def test_rope_refusals(kw, want):
+    r = rope_desc(128, 1e4)
+    for name, v in kw.items():
+        if name == "sections":
+            r.sections[:len(v)] = v
+        else:
+            setattr(r, name, v)
+    assert _lib.load().sfa_rope_desc_check(ctypes.byref(r), 128) == want
+    if want != OK:
+        assert append(rope=r) == want
+
+
+def test_rope_check_without_a_rotation():
+    assert _lib.load().sfa_rope_desc_check(None, 128) == BAD
+
+
+def decode(kv=None, **kw):
+    a = dict(q=P, out=P, table=P, mp=4, lens=P, window=64, sink=4, B=2, most=500, scale=0.1, ws=P, size=1 << 30)
+    a.update(kw)
+    return _lib.load().sfa_attn_decode_window(kv or desc(), a["q"], a["out"], a["table"], a["mp"], a["lens"], a["window"], a["sink"], a["B"],
+                                              a["most"], a["scale"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(B=0), OK), (dict(B=-1), BAD), (dict(q=None), BAD), (dict(out=None), BAD), (dict(table=None), BAD), (dict(lens=None), BAD),
+    (dict(mp=0), BAD), (dict(window=0), BAD), (dict(window=-3), BAD), (dict(sink=-1), BAD), (dict(most=0), BAD), (dict(scale=0.0), BAD),
+    (dict(scale=float("nan")), BAD), (dict(scale=float("inf")), BAD), (dict(ws=None), BAD), (dict(size=0), BAD), (dict(ws=P + 16), UNS),
+    (dict(q=P + 4), UNS), (dict(out=P + 4), UNS),
+])
+def test_decode_refusals(kw, want):
+    assert decode(**kw) == want
+
+
+def prefill(kv=None, **kw):
+    a = dict(q=P, out=P, table=P, mp=4, pos0=0, T=5, window=64, sink=4, scale=0.1, ws=P, size=1 << 30)
+    a.update(kw)
+    return _lib.load().sfa_attn_prefill_window(kv or desc(), a["q"], a["out"], a["table"], a["mp"], a["pos0"], a["T"], a["window"], a["sink"],
+                                               a["scale"], a["ws"], a["size"], None)
+
+
+@pytest.mark.parametrize("kw,want", [
+    (dict(T=0), OK), (dict(T=-1), BAD), (dict(pos0=-1), BAD), (dict(pos0=MAX, T=1), BAD), (dict(q=None), BAD), (dict(out=None), BAD),
+    (dict(table=None), BAD), (dict(mp=0), BAD), (dict(window=0), BAD), (dict(sink=-1), BAD), (dict(scale=-1.0), BAD),
+    (dict(q=P + 4), UNS), (dict(out=P + 4), UNS),
+])
+def test_prefill_refusals(kw, want):
+    assert prefill(**kw) == want
+
+
+def test_descriptor_refusals():
+    for kv, want in ((desc(head_dim=96), UNS), (desc(n_head=24), UNS), (desc(n_head=30), BAD), (desc(page_size=40), BAD),
+                     (desc(kv_type=_lib.SFA_KV_Q8_0, head_dim=32), UNS), (desc(kv_type=2), UNS)):
+        assert decode(kv=kv) == want and prefill(kv=kv) == want and append(kv=kv) == want
+    assert prefill(kv=desc(page_size=32)) == UNS
+    assert decode(kv=desc(page_size=32), B=0) == OK
+
+
+def test_workspace_sizes():
+    lib = _lib.load()
+    for bad in ((0, 500, 64, 4), (2, 0, 64, 4), (2, 500, 0, 4), (2, 500, 64, -1)):
+        assert lib.sfa_decode_window_workspace_bytes(desc(), *bad) == 0
+    need = lib.sfa_decode_window_workspace_bytes(desc(), 2, 500, 64, 4)
+    assert need > 0 and decode(size=need - 1) == BAD
+    # a call's need does not grow with what it cannot attend
+    assert lib.sfa_decode_window_workspace_bytes(desc(), 2, MAX, 64, 4) <= lib.sfa_decode_window_workspace_bytes(desc(), 2, MAX, MAX, MAX) < 1 << 30
+    for bad in ((-1, 5, 64, 4), (0, 0, 64, 4), (0, 5, 0, 4), (0, 5, 64, -1), (MAX, 5, 64, 4)):
+        assert lib.sfa_prefill_window_workspace_bytes(desc(), *bad) == 0
