@@ -6,24 +6,12 @@
 // running maximum and sum of the softmax.
 #include <exception>
 
-#include "sfa_common.h"
-#include "sfa_window.h"
+#include "sfa_window_dev.h"
 
 namespace sfa {
 
-struct WindowParams {
-    const float *q;
-    float *out;
-    const uint8_t *k_pages, *v_pages, *k_cold, *v_cold;
-    int64_t page_bytes;
-    int n_pages, n_cold, page_size, max_pages;
-    int n_head, n_head_kv, row_bytes;
-    const int32_t *page_table;
-    const int32_t *seq_len;  // decode; null for a chunk
-    int q_pos0;              // chunk
-    int window, n_sink;
-    float scale_log2;        // scale * log2(e): probabilities are powers of two
-};
+int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink);
+int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s);
 
 // What one token attends: [0, ns) and [lo, hi].
 struct Span {
@@ -62,11 +50,9 @@ __global__ __launch_bounds__(256) void window_simple_kernel(WindowParams p) {
     for (int i = threadIdx.x; i < G * HD; i += 256)
         qs[i / HD][i % HD] = p.q[((int64_t)t * p.n_head + kvh * G) * HD + i] * p.scale_log2;
     __syncthreads();
-    const int b = p.seq_len != nullptr ? t : 0;
-    const int pos = p.seq_len != nullptr ? p.seq_len[t] - 1 : p.q_pos0 + t;
-    const Span sp = span_of(p, pos);
-    const int n = pos < 0 ? 0 : sp.count();
-    const int32_t *table = p.page_table + (int64_t)b * p.max_pages;
+    const Span sp = span_of(p, p.q_pos0 + t);
+    const int n = sp.count();
+    const int32_t *table = p.page_table;
     float m[G], l[G], o[G][D];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -198,6 +184,16 @@ static int window_args(const sfa_kv_desc *kv, const float *q, float *out, const 
     return SFA_OK;
 }
 
+// Split records of `rows` rows in a workspace: the outputs, then the statistics.
+static size_t records_bytes(int64_t rows, int n_split, int head_dim) {
+    return n_split == 1 ? 256 : (size_t)rows * n_split * (head_dim + 2) * sizeof(float);
+}
+static void set_records(WindowParams *p, void *workspace, int64_t rows, int n_split, int head_dim) {
+    p->n_split = n_split;
+    p->rec_o = static_cast<float *>(workspace);
+    p->rec_ml = reinterpret_cast<float2 *>(p->rec_o + rows * n_split * head_dim);
+}
+
 static int window_launch(const sfa_kv_desc *kv, const WindowParams &p, int n_rows, hipStream_t stream) {
     switch (kv->kv_type) {
     case SFA_KV_F32: return launch_hd<SFA_KV_F32>(p, kv->head_dim, n_rows, stream);
@@ -214,7 +210,8 @@ extern "C" {
 SFA_API size_t sfa_decode_window_workspace_bytes(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len,
                                                  int32_t window, int32_t n_sink) {
     if (sfa_kv_desc_check(kv) != SFA_OK || B <= 0 || max_seq_len <= 0 || window <= 0 || n_sink < 0) return 0;
-    return 256;
+    return sfa::records_bytes((int64_t)B * kv->n_head, sfa::window_decode_splits(kv, B, max_seq_len, window, n_sink),
+                              kv->head_dim);
 }
 
 SFA_API int sfa_attn_decode_window(const sfa_kv_desc *kv, const float *q, float *out,
@@ -235,7 +232,9 @@ SFA_API int sfa_attn_decode_window(const sfa_kv_desc *kv, const float *q, float 
         if (ws_bytes < sfa_decode_window_workspace_bytes(kv, B, max_seq_len, window, n_sink))
             return SFA_ERR_INVALID_ARGUMENT;
         p.seq_len = seq_len;
-        return sfa::window_launch(kv, p, B, static_cast<hipStream_t>(stream));
+        sfa::set_records(&p, workspace, (int64_t)B * kv->n_head,
+                         sfa::window_decode_splits(kv, B, max_seq_len, window, n_sink), kv->head_dim);
+        return sfa::window_decode_launch(p, kv, B, static_cast<hipStream_t>(stream));
     } catch (...) {
         return SFA_ERR_RUNTIME;
     }

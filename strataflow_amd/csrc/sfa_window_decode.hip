@@ -1,0 +1,521 @@
+// sfa_window_decode.hip - one new token per sequence over a sliding window and
+// the sinks (sfa_attn_decode_window, include/sfa_window.h).
+//
+// Bound by memory: a sequence's visible K and V rows are read once.  They are
+// cut into tiles of 4 KB to 8 KB a tensor; a wave streams its tiles through
+// two LDS buffers of its own (asynchronous loads, the next tile under way
+// while one is computed), with the running maximum and sum of the softmax, and
+// the waves of a workgroup, then the workgroups of a sequence (the merge
+// kernel), join their (maximum, sum, output).
+//
+// S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions: their 16 columns
+// are the G query heads of a kv head, and lane l holds column l % 16 of both,
+// so that a score becomes the operand of the second product in the lane that
+// has it.  Q and P keep 32 bits: F32 caches multiply in f32; F16 and Q8_0
+// caches, whose values f16 holds (a quant is one, its block's scale is kept
+// apart), multiply by Q and P as two f16 each.  These kernels wait for memory,
+// so the second product costs them nothing.
+#include "sfa_window_dev.h"
+
+namespace sfa {
+
+constexpr int kWaves = 4;
+
+// Positions of a tile and its bytes in LDS.
+template <int KVT, int HD>
+struct Tile {
+    static constexpr int TP = KVT == SFA_KV_F32 ? 16 : 32;
+    static constexpr int RB = KVT == SFA_KV_F32 ? HD * 4 : KVT == SFA_KV_F16 ? HD * 2 : HD / kQK * kQ8Bytes;
+    static constexpr int CPR = (RB + 15) / 16;               // 16-byte chunks of a row (Q8_0 rows end inside one)
+    static constexpr int ROW = CPR * 16;                     // row in LDS
+    static constexpr int NI = (TP * CPR + kWave - 1) / kWave;  // load instructions
+    static constexpr int BYTES = NI * 1024;
+    static constexpr int RP = 256 / ROW > 0 ? 256 / ROW : 1;  // rows under all LDS banks (a power of two but for Q8_0)
+};
+
+// Where chunk j of row r lies in its LDS row.  The reads of 16 rows at one
+// chunk (K) and of 8 rows at two neighbouring chunks (V of F16) or 4 rows at
+// four (V of F32) then cover the banks evenly.
+template <int KVT, int HD>
+__device__ inline int k_slot(int r, int j) {
+    if constexpr (KVT == SFA_KV_Q8_0) return j;
+    using T = Tile<KVT, HD>;
+    return j ^ (r / T::RP % (T::CPR < 16 ? T::CPR : 16));
+}
+template <int KVT, int HD>
+__device__ inline int v_slot(int r, int j) {
+    using T = Tile<KVT, HD>;
+    if constexpr (KVT == SFA_KV_F16) return j ^ (r / T::RP % (T::CPR / 2) * 2);
+    if constexpr (KVT == SFA_KV_F32) return j ^ (r / 4 % (T::CPR / 4) * 4);
+    return j;
+}
+
+// 8 quants at a 2-byte aligned LDS address as f16 (exact): byte b is 1024 +
+// (b + 128) under the exponent of 1024.
+__device__ inline half2v quants2(uint32_t two) {  // bytes 0 and 2
+    const half2v base = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(half2v, two ^ 0x64806480u) - base;
+}
+__device__ inline half8 quants8(uint32_t a, uint32_t b) {
+    half8 r;
+    const half2v h[4] = {quants2(__builtin_amdgcn_perm(0, a, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, a, 0x0c030c02)),
+                         quants2(__builtin_amdgcn_perm(0, b, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, b, 0x0c030c02))};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[2 * i] = h[i][0], r[2 * i + 1] = h[i][1];
+    return r;
+}
+
+template <int KVT, int HD, int G>
+__global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowParams p) {
+    using T = Tile<KVT, HD>;
+    constexpr int TP = T::TP, MT = TP / 16;  // 16-position blocks of a tile
+    constexpr int KS = HD / 32, DB = HD / 16;
+    constexpr int NB = HD / kQK;             // quantisation blocks of a row
+    constexpr int STAGE = 2 * T::BYTES;
+    constexpr int TAB = KVT == SFA_KV_Q8_0 ? 2 * NB * TP * 4 : 0;  // a wave's scales of the tile, K and V
+    constexpr int WAVE = 2 * STAGE + TAB;
+    constexpr int JOIN = (int)sizeof(float) * kWaves * G * (HD + 2);
+    __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * WAVE > JOIN ? kWaves * WAVE : JOIN];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, qd = lane >> 4;
+    const int kvh = blockIdx.x % p.n_head_kv;
+    const int rest = blockIdx.x / p.n_head_kv;
+    const int split = rest % p.n_split, b = rest / p.n_split;
+    const int32_t *table = p.page_table + (int64_t)b * p.max_pages;
+    const int len = p.seq_len[b];
+
+    // Q of column c: rows past G are zero columns
+    float amax = 0.0f;
+    float qx[KS][8];
+    const float *qrow = p.q + ((int64_t)b * p.n_head + kvh * G + (c < G ? c : 0)) * HD;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        // F32: dims 16 j + 4 qd of chunk j = 2 ks and 2 ks + 1; else dims 32 ks + 8 qd
+        const int d0 = KVT == SFA_KV_F32 ? 32 * ks + 4 * qd : 32 * ks + 8 * qd;
+        const int d1 = KVT == SFA_KV_F32 ? d0 + 16 : d0 + 4;
+        const floatx4 u = *reinterpret_cast<const floatx4 *>(qrow + d0);
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(qrow + d1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            qx[ks][j] = c < G ? u[j] : 0.0f;
+            qx[ks][4 + j] = c < G ? v[j] : 0.0f;
+        }
+    }
+
+    // what the token attends: [0, ns) and [lo, hi], as tiles: the first n_sink
+    // ones, then those of the window
+    const int64_t cap = (int64_t)p.max_pages * p.page_size;
+    const int pos = len - 1;
+    const int lo = pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
+    const int hi = pos < cap ? pos : (int)(cap - 1);
+    const int ns = min(min(p.n_sink, lo), hi + 1);
+    const int sink_tiles = pos < 0 ? 0 : (ns + TP - 1) / TP;
+    const int n_tiles = pos < 0 ? 0 : sink_tiles + (hi >= lo ? hi / TP - lo / TP + 1 : 0);
+    const int t0 = (int)((int64_t)n_tiles * split / p.n_split);
+    const int t1 = (int)((int64_t)n_tiles * (split + 1) / p.n_split);
+
+    const int col_bytes = p.n_head_kv * T::RB;
+    int k_off[T::NI], v_off[T::NI];
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) {
+        const int ch = 64 * i + lane, r = ch / T::CPR, j = ch % T::CPR;
+        const bool in = ch < TP * T::CPR;  // the rest of the last instruction loads nothing
+        k_off[i] = in ? r * col_bytes + 16 * k_slot<KVT, HD>(r, j) : -(1 << 30);
+        v_off[i] = in ? r * col_bytes + 16 * v_slot<KVT, HD>(r, j) : -(1 << 30);
+    }
+    uint8_t *const mine = lds + wave * WAVE;
+    const uint32_t mine_at = lds_addr(mine);
+    PageWindow pages;
+    int r0[2], r1[2];  // visible rows of the tile in each buffer
+    auto issue = [&](int t, int buf) {
+        const bool sink = t < sink_tiles;
+        const int first = (sink ? t : lo / TP + t - sink_tiles) * TP;
+        const int from = max(sink ? 0 : lo - first, 0), to = min((sink ? ns : hi + 1) - first, TP);
+        const int lp = first / p.page_size;
+        const int32_t id = pages.get(table, p.max_pages, lp, lane);
+        const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
+        const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
+        const bool there = kb != nullptr && vb != nullptr;
+        // the buffer holds the visible rows alone: what else the tile's place in
+        // the page holds is not read
+        const int64_t row = (int64_t)(first - lp * p.page_size + from) * col_bytes + kvh * T::RB;
+        const int bytes = there ? (to - from - 1) * col_bytes + T::RB : 0;
+        const auto kr = buffer_of(there ? kb + row : nullptr, bytes);
+        const auto vr = buffer_of(there ? vb + row : nullptr, bytes);
+        const int up = from * col_bytes;
+        const uint32_t at = mine_at + buf * STAGE;
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i) load_to_lds(kr, at + 1024 * i, k_off[i] - up);
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i) load_to_lds(vr, at + T::BYTES + 1024 * i, v_off[i] - up);
+        r0[buf] = from;
+        r1[buf] = there ? to : 0;
+    };
+    int t = t0 + wave;
+    if (t < t1) {
+        pages.load(table, p.max_pages, (t < sink_tiles ? t * TP : (lo / TP + t - sink_tiles) * TP) / p.page_size, lane);
+        issue(t, 0);
+    }
+
+    // Q as two f16 under a power of two of its row, or as it is
+    float up = 1.0f;
+    half8 qh[KS], ql[KS];
+    if constexpr (KVT != SFA_KV_F32) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[ks][j]));
+        float down;
+        row_exponent(quarters_max(amax), down, up);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 h, l;
+                split_f16(qx[ks][j] * down, h, l);
+                qh[ks][j] = h;
+                ql[ks][j] = l;
+            }
+    }
+    const float f = p.scale_log2 * up;
+
+    // probabilities are 2^(s f - base), base kSplitShift below the column's
+    // running maximum (F32: at it); l sums this lane's
+    constexpr float SHIFT = KVT == SFA_KV_F32 ? 0.0f : (float)kSplitShift;
+    float base = -INFINITY, l = 0.0f;
+    // Q8_0: V's scales are taken down by the power of two of the largest so far,
+    // in whose units o is: a probability times a scale fits an f16 then
+    int unit = 1;
+    floatx4 o[DB];                  // O^T: dims 16 db + 4 qd + i (Q8_0: see there) of column c
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    int buf = 0;
+    for (; t < t1; t += kWaves, buf ^= 1) {
+        // the reads of this buffer's last tile are done before it is filled again
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + kWaves < t1) {
+            issue(t + kWaves, buf ^ 1);
+            wait_loads<2 * T::NI>();
+        } else {
+            wait_loads<0>();
+        }
+        const uint8_t *const ks0 = mine + buf * STAGE, *const vs0 = ks0 + T::BYTES;
+        floatx4 s[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (KVT == SFA_KV_F16) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const int r = 16 * mt + c;
+                    const half8 a = *reinterpret_cast<const half8 *>(ks0 + r * T::ROW + 16 * k_slot<KVT, HD>(r, 4 * ks + qd));
+                    s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[ks], s[mt], 0, 0, 0);
+                    s[mt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[ks], s[mt], 0, 0, 0);
+                }
+        } else if constexpr (KVT == SFA_KV_F32) {
+#pragma unroll
+            for (int ks = 0; ks < 2 * KS; ++ks) {
+                const floatx4 a = *reinterpret_cast<const floatx4 *>(ks0 + c * T::ROW + 16 * k_slot<KVT, HD>(c, 4 * ks + qd));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], qx[ks / 2][ks % 2 * 4 + i], s[0], 0, 0, 0);
+            }
+        } else {
+            // the blocks' scales, K then V, as f32 [block][position]: a lane needs those of its
+            // eight score rows, whose K rows are other lanes' operands
+            float *const tab = reinterpret_cast<float *>(mine + 2 * STAGE);
+            const int tp = lane & 31;
+            const uint8_t *const src = (lane < 32 ? ks0 : vs0) + tp * T::ROW;
+            float d[NB], dmax = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                d[nb] = (float)*reinterpret_cast<const _Float16 *>(src + kQ8Bytes * nb);
+                dmax = fmaxf(dmax, fabsf(d[nb]));
+            }
+            const int e = max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, wave_max(lane < 32 ? 0.0f : dmax)) >> 23)), 1);
+            if (e > unit) {
+                const float a = __builtin_amdgcn_ldexpf(1.0f, unit - e);
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[i] *= a;
+                unit = e;
+            }
+            const float down = lane < 32 ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, 127 - unit);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) tab[(lane < 32 ? 0 : NB * TP) + nb * TP + tp] = d[nb] * down;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint8_t *const blk = ks0 + (16 * mt + c) * T::ROW + kQ8Bytes * nb + 2 + 8 * qd;
+                    uint32_t w[3];
+                    half8 a;
+                    if (nb % 2) {  // the quants of odd blocks start at a multiple of 4, those of even ones 2 after one
+                        __builtin_memcpy(w, __builtin_assume_aligned(blk, 4), 8);
+                        a = quants8(w[0], w[1]);
+                    } else {
+                        __builtin_memcpy(w, __builtin_assume_aligned(blk - 2, 4), 12);
+                        a = quants8(__builtin_amdgcn_alignbyte(w[1], w[0], 2), __builtin_amdgcn_alignbyte(w[2], w[1], 2));
+                    }
+                    floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[nb], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[nb], x, 0, 0, 0);
+                    const floatx4 d = *reinterpret_cast<const floatx4 *>(tab + nb * TP + 16 * mt + 4 * qd);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(x[i], d[i], s[mt][i]);
+                }
+        }
+        const int from = r0[buf], to = r1[buf];
+        if (from > 0 || to < TP) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 16 * mt + 4 * qd + i;
+                    if (r < from || r >= to) s[mt][i] = -INFINITY;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+            mx = fmaxf(mx, fmaxf(fmaxf(s[mt][0], s[mt][1]), fmaxf(s[mt][2], s[mt][3])));
+        mx = quarters_max(mx) * f - SHIFT;
+        if (__ballot(mx > base) != 0) {
+            const float nb = fmaxf(mx, base);
+            const float a = nb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - nb);
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= a;
+            base = nb;
+        }
+        const float sub = base == -INFINITY ? 0.0f : base;
+        float pr[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pr[mt][i] = __builtin_amdgcn_exp2f(fmaf(s[mt][i], f, -sub));
+                l += pr[mt][i];
+            }
+        if constexpr (KVT == SFA_KV_F32) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * qd + i;
+                    const float a = *reinterpret_cast<const float *>(vs0 + r * T::ROW + 16 * v_slot<KVT, HD>(r, 4 * d + c / 4) + 4 * (c & 3));
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pr[0][i], o[d], 0, 0, 0);
+                }
+        } else if constexpr (KVT == SFA_KV_F16) {
+            half8 ph, pl;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                _Float16 h, lo16;
+                split_f16(pr[j / 4][j % 4], h, lo16);
+                ph[j] = h;
+                pl[j] = lo16;
+            }
+            // operand positions 4 qd .. and 16 + 4 qd ..: the lane's own scores
+            const int rr = 4 * qd + (c >> 2);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const int at = 16 * v_slot<KVT, HD>(rr, 2 * d + ((c & 3) >> 1)) + 8 * (c & 1);
+                const int at2 = 16 * v_slot<KVT, HD>(rr + 16, 2 * d + ((c & 3) >> 1)) + 8 * (c & 1);
+                const half4 x = tr16_read(vs0 + rr * T::ROW + at), y = tr16_read(vs0 + (rr + 16) * T::ROW + at2);
+                const half8 a = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[d], 0, 0, 0);
+            }
+        } else {
+            const float *const tab = reinterpret_cast<const float *>(mine + 2 * STAGE) + NB * TP;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                // a position's block scale goes with its probability
+                half8 ph, pl;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const floatx4 d = *reinterpret_cast<const floatx4 *>(tab + nb * TP + 16 * mt + 4 * qd);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        _Float16 h, lo16;
+                        split_f16(pr[mt][i] * d[i], h, lo16);
+                        ph[4 * mt + i] = h;
+                        pl[4 * mt + i] = lo16;
+                    }
+                }
+                // rows of two products: dims 2 c and 2 c + 1 of the block, one 16-bit read a position
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int ra = j < 2 ? 4 * qd + 2 * j : 16 + 4 * qd + 2 * (j - 2);
+                    const uint8_t *const src = vs0 + ra * T::ROW + kQ8Bytes * nb + 2 + 2 * c;
+                    w[j] = *reinterpret_cast<const uint16_t *>(src) | (uint32_t)*reinterpret_cast<const uint16_t *>(src + T::ROW) << 16;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    half8 a;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const half2v h = quants2((e ? w[j] >> 8 : w[j]) & 0x00ff00ffu);
+                        a[2 * j] = h[0];
+                        a[2 * j + 1] = h[1];
+                    }
+                    o[2 * nb + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[2 * nb + e], 0, 0, 0);
+                    o[2 * nb + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[2 * nb + e], 0, 0, 0);
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+
+    // the four waves join
+    l = quarters_sum(l);
+    if constexpr (KVT == SFA_KV_Q8_0) {
+        const float back = __builtin_amdgcn_ldexpf(1.0f, unit - 127);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] *= back;
+    }
+    float *const jm = reinterpret_cast<float *>(lds), *const jl = jm + kWaves * G, *const jo = jl + kWaves * G;
+    __syncthreads();
+    if (c < G) {
+        if (qd == 0) {
+            jm[wave * G + c] = base;
+            jl[wave * G + c] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = KVT == SFA_KV_Q8_0 ? d / 2 * 32 + 2 * (4 * qd + i) + d % 2 : 16 * d + 4 * qd + i;
+                jo[(wave * G + c) * HD + e] = o[d][i];
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < G * HD; i += 64 * kWaves) {
+        const int g = i / HD;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, jm[w * G + g]);
+        const float mb = mm == -INFINITY ? 0.0f : mm;
+        float L = 0.0f, acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float x = __builtin_amdgcn_exp2f(jm[w * G + g] - mb);
+            L = fmaf(jl[w * G + g], x, L);
+            acc = fmaf(jo[w * G * HD + i], x, acc);
+        }
+        const int64_t row = (int64_t)b * p.n_head + kvh * G + g;
+        if (p.n_split == 1) {
+            p.out[row * HD + i % HD] = L == 0.0f ? 0.0f : acc / L;
+        } else {
+            p.rec_o[(row * p.n_split + split) * HD + i % HD] = acc;
+            if (i % HD == 0) p.rec_ml[row * p.n_split + split] = make_float2(mm, L);
+        }
+    }
+}
+
+// Joins a row's split records: a thread has four dims of every NG-th split.
+template <int HD>
+__global__ __launch_bounds__(256) void window_merge_kernel(WindowParams p) {
+    constexpr int LN = HD / 4, NG = 256 / LN;
+    __shared__ float jm[NG], jl[NG];
+    __shared__ floatx4 jo[NG][LN];
+    const int64_t row = blockIdx.x;
+    const int grp = threadIdx.x / LN, e = threadIdx.x % LN;
+    const float2 *const ml = p.rec_ml + row * p.n_split;
+    const float *const rec = p.rec_o + row * p.n_split * HD;
+    float m = -INFINITY, l = 0.0f;
+    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s = grp; s < p.n_split; s += NG) {
+        const float2 r = ml[s];
+        const floatx4 x = *reinterpret_cast<const floatx4 *>(rec + (int64_t)s * HD + 4 * e);
+        const float mn = fmaxf(m, r.x), mb = mn == -INFINITY ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - mb), w = __builtin_amdgcn_exp2f(r.x - mb);
+        l = fmaf(r.y, w, l * a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], w, o[i] * a);
+        m = mn;
+    }
+    if (e == 0) jm[grp] = m, jl[grp] = l;
+    jo[grp][e] = o;
+    __syncthreads();
+    if (grp != 0) return;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) mm = fmaxf(mm, jm[g]);
+    if (mm == -INFINITY) mm = 0.0f;
+    float L = 0.0f;
+    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const float w = __builtin_amdgcn_exp2f(jm[g] - mm);
+        L = fmaf(jl[g], w, L);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(jo[g][e][i], w, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = L == 0.0f ? 0.0f : acc[i] / L;
+    *reinterpret_cast<floatx4 *>(p.out + row * HD + 4 * e) = acc;
+}
+
+int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipStream_t s) {
+    const dim3 grid((unsigned)rows), block(256);
+    if (head_dim == 128) hipLaunchKernelGGL(window_merge_kernel<128>, grid, block, 0, s, p);
+    else if (head_dim == 64) hipLaunchKernelGGL(window_merge_kernel<64>, grid, block, 0, s, p);
+    else hipLaunchKernelGGL(window_merge_kernel<32>, grid, block, 0, s, p);
+    return hipGetLastError() == hipSuccess ? SFA_OK : SFA_ERR_RUNTIME;
+}
+
+// Workgroups of one sequence and kv head: as many as fill the chip once (one
+// workgroup a CU where a row's two buffers take over half its LDS, else two),
+// at most one per four tiles of the longest span.
+int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink) {
+    const int tp = kv->kv_type == SFA_KV_F32 ? 16 : 32;
+    const int64_t seen = (int64_t)window + n_sink < max_seq_len ? (int64_t)window + n_sink : max_seq_len;
+    const int64_t tiles = (seen + tp - 1) / tp + 2;
+    const int64_t room = kv->head_dim == 128 ? 256 : 512;
+    int64_t n = room / ((int64_t)B * kv->n_head_kv);
+    if (n > (tiles + kWaves - 1) / kWaves) n = (tiles + kWaves - 1) / kWaves;
+    return n < 1 ? 1 : (int)n;
+}
+
+template <int KVT, int HD>
+static void launch_g(const WindowParams &p, unsigned grid, hipStream_t s) {
+    const dim3 block(64 * kWaves);
+    switch (p.n_head / p.n_head_kv) {
+    case 1: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 1>), dim3(grid), block, 0, s, p); break;
+    case 2: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 2>), dim3(grid), block, 0, s, p); break;
+    case 4: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 4>), dim3(grid), block, 0, s, p); break;
+    default: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 8>), dim3(grid), block, 0, s, p); break;
+    }
+}
+
+template <int KVT>
+static int launch_hd(const WindowParams &p, int head_dim, unsigned grid, hipStream_t s) {
+    if (head_dim == 128) launch_g<KVT, 128>(p, grid, s);
+    else if (head_dim == 64) launch_g<KVT, 64>(p, grid, s);
+    else if constexpr (KVT != SFA_KV_Q8_0) launch_g<KVT, 32>(p, grid, s);
+    else return SFA_ERR_UNSUPPORTED;
+    return hipGetLastError() == hipSuccess ? SFA_OK : SFA_ERR_RUNTIME;
+}
+
+int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s) {
+    const int64_t grid = (int64_t)B * kv->n_head_kv * p.n_split, rows = (int64_t)B * kv->n_head;
+    if (grid > INT32_MAX || rows > INT32_MAX) return SFA_ERR_UNSUPPORTED;
+    int rc;
+    switch (kv->kv_type) {
+    case SFA_KV_F32: rc = launch_hd<SFA_KV_F32>(p, kv->head_dim, (unsigned)grid, s); break;
+    case SFA_KV_F16: rc = launch_hd<SFA_KV_F16>(p, kv->head_dim, (unsigned)grid, s); break;
+    case SFA_KV_Q8_0: rc = launch_hd<SFA_KV_Q8_0>(p, kv->head_dim, (unsigned)grid, s); break;
+    default: return SFA_ERR_UNSUPPORTED;
+    }
+    if (rc != SFA_OK || p.n_split == 1) return rc;
+    return window_merge_launch(p, kv->head_dim, rows, s);
+}
+
+}  // namespace sfa

@@ -1,0 +1,109 @@
+// sfa_window_dev.h - parameters and device helpers of the windowed attention
+// kernels (sfa_window_decode.hip, sfa_window_prefill.hip).
+#pragma once
+
+#include "sfa_common.h"
+#include "sfa_window.h"
+
+namespace sfa {
+
+// Both factors that are split into two f16 are scaled up first, the row of
+// queries and the probabilities to 2^14: the lower half of a value 2^17 times
+// smaller than the largest is a normal f16 then (the matrix cores need not
+// keep subnormal ones).
+constexpr int kSplitShift = 14;
+
+struct WindowParams {
+    const float *q;
+    float *out;
+    const uint8_t *k_pages, *v_pages, *k_cold, *v_cold;
+    int64_t page_bytes;
+    int n_pages, n_cold, page_size, max_pages;
+    int n_head, n_head_kv, row_bytes;
+    const int32_t *page_table;
+    const int32_t *seq_len;  // decode; null for a chunk
+    int q_pos0, n_tok;       // chunk
+    int window, n_sink;
+    float scale_log2;        // scale * log2(e): probabilities are powers of two
+    int n_split;
+    float *rec_o;            // split records: outputs [row][split][HD] not yet divided,
+    float2 *rec_ml;          // and (running maximum, sum) [row][split]
+};
+
+// A raw buffer over [base, base + bytes): loads outside it give zeros, also
+// those at "negative" offsets, which are large unsigned ones.
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, kBufferRsrcWord3);
+}
+
+__device__ inline uint32_t lds_addr(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)p;
+}
+
+// 16 bytes a lane from a buffer straight into LDS at lds_base + 16 * lane.
+// The compiler does not count these loads: the caller waits with wait_loads
+// before it reads what they wrote.  M0 holds the LDS base.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // "m0 is reserved": the kernels use M0 for nothing else
+__device__ inline void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t lds_base, int offset) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(lds_base), "v"(offset), "s"(rsrc)
+        : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Waits until at most N of the wave's loads are in flight (they end in order).
+template <int N>
+__device__ inline void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Maximum and sum over the lanes l % 16 + {0, 16, 32, 48}, in all four.
+__device__ inline void swap_rows16(float x, float &a, float &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x),
+                                                    false, false);
+    static_assert(sizeof(r) == 8, "two 32-bit values");
+    unsigned u0, u1;
+    __builtin_memcpy(&u0, reinterpret_cast<const char *>(&r), 4);
+    __builtin_memcpy(&u1, reinterpret_cast<const char *>(&r) + 4, 4);
+    a = __builtin_bit_cast(float, u0);
+    b = __builtin_bit_cast(float, u1);
+}
+__device__ inline float quarters_max(float x) {
+    float a, b;
+    swap_rows16(x, a, b);
+    x = fmaxf(a, b);
+    swap_halves(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ inline float quarters_sum(float x) {
+    float a, b;
+    swap_rows16(x, a, b);
+    x = a + b;
+    swap_halves(x, a, b);
+    return a + b;
+}
+
+// x as two f16: hi its nearest, lo the nearest of what is left.  The empty asm
+// keeps a product that x comes from out of the conversions: fused with one of
+// them only, it gave a hi and a lo of two different roundings now and then.
+__device__ inline void split_f16(float x, _Float16 &hi, _Float16 &lo) {
+    asm("" : "+v"(x));
+    hi = (_Float16)x;
+    lo = (_Float16)(x - (float)hi);
+}
+
+// Power of two that takes a row's largest value into [2^14, 2^15), and its
+// inverse.
+__device__ inline void row_exponent(float amax, float &down, float &up) {
+    int e = (int)(__builtin_bit_cast(uint32_t, amax) >> 23) & 255;
+    e = e < kSplitShift + 2 ? kSplitShift + 2 : e > 252 ? 252 : e;  // zeros and the ends of the range
+    down = __builtin_bit_cast(float, (uint32_t)(254 + kSplitShift - e) << 23);
+    up = __builtin_bit_cast(float, (uint32_t)(e - kSplitShift) << 23);
+}
+
+}  // namespace sfa
