@@ -30,10 +30,30 @@ struct WindowParams {
     float2 *rec_ml;          // and (running maximum, sum) [row][split]
 };
 
+int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink);
+int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s);
+int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int32_t window, int32_t n_sink);
+int window_prefill_launch(const WindowParams &p, const sfa_kv_desc *kv, hipStream_t s);
+int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipStream_t s);
+
+// x, the same in every lane, in a scalar register.  Without the empty asm the
+// compiler drops the readfirstlane of a value that it knows to be uniform and
+// may keep what follows in vector registers, where the operands of load_to_lds
+// cannot be.
+__device__ inline uint32_t to_scalar(uint32_t x) {
+    asm("" : "+v"(x));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
 // A raw buffer over [base, base + bytes): loads outside it give zeros, also
 // those at "negative" offsets, which are large unsigned ones.
 __device__ inline __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *base, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, kBufferRsrcWord3);
+    const uint64_t u = reinterpret_cast<uint64_t>(base);
+    uint32_t lo = to_scalar((uint32_t)u), hi = to_scalar((uint32_t)(u >> 32)), n = to_scalar((uint32_t)bytes);
+    // a load may read a scalar register five states after a vector instruction
+    // wrote it, and the compiler does not see the load in load_to_lds
+    asm volatile("s_nop 4" : "+s"(lo), "+s"(hi), "+s"(n));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>((uint64_t)hi << 32 | lo), 0, (int)n, kBufferRsrcWord3);
 }
 
 __device__ inline uint32_t lds_addr(const void *p) {

@@ -183,23 +183,57 @@ def test_prefill_peaks(gpu, kv_type):
     run_prefill(c, 700, 512, 4)
 
 
-@pytest.mark.parametrize("kv_type", [F32, F16])
+@pytest.mark.parametrize("kv_type,hd", [(F32, 64), (F16, 64), (Q8, 64), (Q8, 128)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("past,T", [(0, 40), (200, 300)])
-def test_prefill_masked_values_have_no_part(gpu, kv_type, bad, past, T):
-    """A row whose K and V are not finite: tokens that may not see it are as without it."""
+def test_prefill_masked_values_have_no_part(gpu, kv_type, hd, bad, past, T):
+    """A row whose K and V are not finite: tokens that may not see it are as without it, the others NaN."""
     W, at = 50, past + T // 2
-    c = Cache(lens=[past + T], kv_type=kv_type, seed=11)
+    c = Cache(lens=[past + T], kv_type=kv_type, head_dim=hd, seed=11)
     dt = torch.float32 if kv_type == F32 else torch.float16
     page = int(c.table[0, at // c.ps])
     for pool in (c.kv.k, c.kv.v):
-        pool[0, page].view(dt).view(c.ps, c.Hkv, c.hd)[at % c.ps] = bad
+        rows = pool[0, page].view(c.ps, c.Hkv, -1)[at % c.ps]
+        if kv_type == Q8:
+            rows = rows.view(c.Hkv, hd // 32, 34)[..., :2]  # the blocks' scales
+            rows.copy_(torch.full((1,), bad, dtype=dt).cuda().view(torch.uint8).expand_as(rows))
+        else:
+            rows.copy_(torch.full((1, hd), bad, dtype=dt).cuda().view(torch.uint8).expand_as(rows))
     q = c.queries(T)
     out = c.kv.prefill_window(0, cuda(q), c.t_table[0], past, W, 3)
     t = np.arange(past, past + T)
     free = (t < at) | (t >= at + W)
     want, bound = c.attend(0, q, t, W, 3)
     check(out[torch.from_numpy(free).cuda()], want[free], bound[free], c.hd)
+    assert torch.isnan(out[torch.from_numpy(~free).cuda()]).all()
+
+
+@pytest.mark.parametrize("kv_type", [F32, F16, Q8])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_prefill_masked_values_alone(gpu, kv_type, bad):
+    """V alone not finite: the dims that it has of the rows that see it are not finite, nothing else is."""
+    past, T, W, at = 100, 120, 50, 150
+    c = Cache(lens=[past + T], kv_type=kv_type, head_dim=64, seed=12)
+    dt = torch.float32 if kv_type == F32 else torch.float16
+    rows = c.kv.v[0, int(c.table[0, at // c.ps])].view(c.ps, c.Hkv, -1)[at % c.ps]
+    dims = np.zeros(64, bool)
+    dims[32 if kv_type == Q8 else 37] = True
+    if kv_type == Q8:
+        dims[32:] = True
+        rows.view(c.Hkv, 2, 34)[0, 1, :2] = torch.full((1,), bad, dtype=dt).cuda().view(torch.uint8)
+    else:
+        rows.view(dt)[0, 37] = bad
+    q = c.queries(T)
+    out = c.kv.prefill_window(0, cuda(q), c.t_table[0], past, W, 3)
+    t = np.arange(past, past + T)
+    want, bound = c.attend(0, q, t, W, 3)
+    hit = np.zeros((T, c.Hq, 64), bool)
+    hit[(t >= at) & (t < at + W), :c.Hq // c.Hkv] = dims
+    hit = hit.reshape(T, -1)
+    out = out.cpu().numpy()
+    assert not np.isfinite(out[hit]).any()
+    off = np.abs(np.where(hit, want, out) - want)
+    assert (off <= bound).all()
 
 
 # ---- append ----------------------------------------------------------------------------------------------
