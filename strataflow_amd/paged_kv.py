@@ -9,7 +9,6 @@ tensors, so a call does no host-to-device copy.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -62,21 +61,19 @@ def _stream(stream) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def _on(device: torch.device):
-    """The device current for a call, where it is another one."""
-    if device.index in (None, torch.cuda.current_device()):
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _raw_stream(stream, device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else _stream(stream)
 
 
-def _empty(shape: tuple, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
-    """An uninitialised tensor in the allocator's order of the stream that uses
-    it: freed while the call still runs, it is handed on to that stream alone."""
+def _empty(shape: tuple, like: torch.Tensor, stream, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """An uninitialised tensor on `like`'s device (and of its type) in the
+    allocator's order of the stream that uses it: freed while the call still
+    runs, it is handed on to that stream alone."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(_stream(stream), device)
+        return like.new_empty(shape, dtype=dtype)
+    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(_stream(stream), like.device)
     with torch.cuda.stream(s):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 class PagedKV:
@@ -93,6 +90,8 @@ class PagedKV:
         self.k = torch.zeros((n_layer, n_pages, self.page_bytes), dtype=torch.uint8, device=self.device)
         self.v = torch.zeros_like(self.k)
         self._dev = self.k.device  # with its index
+        self._index = self.k.get_device()
+        self._scale = self.scale
         if n_cold_pages:
             # host-pinned cold pool, readable by the GPU over the host link
             self.k_cold = torch.zeros((n_layer, n_cold_pages, self.page_bytes), dtype=torch.uint8,
@@ -102,6 +101,7 @@ class PagedKV:
             self.k_cold = self.v_cold = None
         self._ws = None
         self._ws_need = {}
+        self._ws_window = {}
         self._descs = [self._make_desc(layer) for layer in range(n_layer)]
         lib = _lib.load()
         _lib.check(lib.sfa_kv_desc_check(ctypes.byref(self.desc(0))), "kv descriptor")
@@ -264,16 +264,14 @@ class PagedKV:
         return out
 
     # -- windowed models: head norms and rotations on the append, window + sinks ----
-    def _is(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple | None = None) -> torch.Tensor:
-        if t.dtype is not dtype or t.device != self._dev or not t.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous {dtype} tensor on {self._dev}")
-        if shape is not None and t.shape != shape:
-            raise ValueError(f"{what} has shape {tuple(t.shape)}, not {shape}")
-        return t
+    # (the checks are spelled out: where a launch takes 4 us, a helper call per
+    # tensor would take as much again)
+    def _bad(self, what: str, dtype: str, shape: str) -> ValueError:
+        return ValueError(f"{what} must be a contiguous {dtype} tensor {shape} on {self._dev}")
 
     def _heads(self, t: torch.Tensor, what: str, n_tok: int, heads: int) -> int:
         """Checks [n_tok, heads, hd] f32 rows, whole within a token; the stride between tokens."""
-        if t.dtype is not torch.float32 or t.device != self._dev or t.shape != (n_tok, heads, self.head_dim):
+        if t.dtype is not torch.float32 or t.get_device() != self._index or t.shape != (n_tok, heads, self.head_dim):
             raise ValueError(f"{what} must be float32 [{n_tok}, {heads}, {self.head_dim}] on {self._dev}")
         step, head, one = t.stride()
         if one != 1 or (heads > 1 and head != self.head_dim):
@@ -291,32 +289,61 @@ class PagedKV:
         q [n_tok, Hq, hd] (or None), k, v [n_tok, Hkv, hd] f32 may be slices of
         the stacked Q/K/V rows; rope_pos [n_axis, n_tok] int32 (default: pos on
         every axis)."""
+        i32, dev, hd = torch.int32, self._index, self.head_dim
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.norm_rope_append(layer, q, k, v, seq, pos, page_table, rope, q_norm, k_norm, eps, rope_pos,
+                                             q_out, stream)
         n_tok = seq.numel()
         ks = self._heads(k, "k", n_tok, self.n_head_kv)
         vs = self._heads(v, "v", n_tok, self.n_head_kv)
-        self._is(seq, "seq", torch.int32)
-        self._is(pos, "pos", torch.int32, seq.shape)
-        self._is(page_table, "page_table", torch.int32)
-        qs = 0
+        if seq.dtype is not i32 or seq.get_device() != dev or not seq.is_contiguous():
+            raise self._bad("seq", "int32", "[n_tok]")
+        if pos.dtype is not i32 or pos.get_device() != dev or not pos.is_contiguous() or pos.numel() != n_tok:
+            raise self._bad("pos", "int32", f"[{n_tok}]")
+        if page_table.dtype is not i32 or page_table.get_device() != dev or not page_table.is_contiguous():
+            raise self._bad("page_table", "int32", "[n_seq, max_pages]")
+        qs, qp, op = 0, None, None
         if q is not None:
-            qs = self._heads(q, "q", n_tok, self.n_head)
+            qs, qp = self._heads(q, "q", n_tok, self.n_head), q.data_ptr()
             if q_out is None:
-                q_out = _empty((n_tok, self.n_head, self.head_dim), torch.float32, self._dev, stream)
-            else:
-                self._is(q_out, "q_out", torch.float32, (n_tok, self.n_head, self.head_dim))
+                q_out = _empty((n_tok, self.n_head, hd), q, stream)
+            elif self._heads(q_out, "q_out", n_tok, self.n_head) != self.n_head * hd and n_tok > 1:
+                raise self._bad("q_out", "float32", f"[{n_tok}, {self.n_head}, {hd}]")
+            op = q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None:
-                self._is(w, what, torch.float32, (self.head_dim,))
+        wq = wk = rp = None
+        if q_norm is not None:
+            if q_norm.dtype is not torch.float32 or q_norm.get_device() != dev or q_norm.shape != (hd,) or not q_norm.is_contiguous():
+                raise self._bad("q_norm", "float32", f"[{hd}]")
+            wq = q_norm.data_ptr()
+        if k_norm is not None:
+            if k_norm.dtype is not torch.float32 or k_norm.get_device() != dev or k_norm.shape != (hd,) or not k_norm.is_contiguous():
+                raise self._bad("k_norm", "float32", f"[{hd}]")
+            wk = k_norm.data_ptr()
         if rope_pos is not None:
-            self._is(rope_pos, "rope_pos", torch.int32, (rope.n_axis, n_tok))
-        with _on(self._dev):
-            _lib.check(_lib.load().sfa_norm_rope_kv_append(
-                self._descs[layer], rope, _ptr(q), qs, _ptr(q_out), k.data_ptr(), ks, v.data_ptr(), vs, _ptr(q_norm),
-                _ptr(k_norm), eps, seq.data_ptr(), pos.data_ptr(), _ptr(rope_pos), n_tok, page_table.data_ptr(),
-                page_table.shape[-1], _stream(stream)), "sfa_norm_rope_kv_append")
+            if (rope_pos.dtype is not i32 or rope_pos.get_device() != dev or not rope_pos.is_contiguous()
+                    or rope_pos.shape != (rope.n_axis, n_tok)):
+                raise self._bad("rope_pos", "int32", f"[{rope.n_axis}, {n_tok}]")
+            rp = rope_pos.data_ptr()
+        rc = _lib.load().sfa_norm_rope_kv_append(
+            self._descs[layer], rope, qp, qs, op, k.data_ptr(), ks, v.data_ptr(), vs, wq, wk, eps, seq.data_ptr(),
+            pos.data_ptr(), rp, n_tok, page_table.data_ptr(), page_table.shape[-1], _raw_stream(stream, dev))
+        if rc:
+            _lib.check(rc, "sfa_norm_rope_kv_append")
         return q_out
+
+    def _rows(self, q: torch.Tensor, out: torch.Tensor | None, n: int, stream) -> torch.Tensor:
+        """Checks q [n, Hq, hd] and out [n, Hq*hd]; out, a new one by default."""
+        Hq, hd = self.n_head, self.head_dim
+        if q.dtype is not torch.float32 or q.get_device() != self._index or q.shape != (n, Hq, hd) or not q.is_contiguous():
+            raise self._bad("q", "float32", f"[{n}, {Hq}, {hd}]")
+        if out is None:
+            return _empty((n, Hq * hd), q, stream)
+        if out.dtype is not torch.float32 or out.get_device() != self._index or out.shape != (n, Hq * hd) or not out.is_contiguous():
+            raise self._bad("out", "float32", f"[{n}, {Hq * hd}]")
+        return out
 
     def decode_window(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, seq_len: torch.Tensor,
                       max_seq_len: int, window: int, n_sink: int = 0, out: torch.Tensor | None = None,
@@ -324,21 +351,30 @@ class PagedKV:
         """q [B, Hq, hd] f32 -> out [B, Hq*hd] f32: the token at seq_len[b] - 1
         attends the last ``window`` positions and the first ``n_sink``.  The
         workspace is the call's own."""
+        i32, dev = torch.int32, self._index
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.decode_window(layer, q, page_table, seq_len, max_seq_len, window, n_sink, out, scale, stream)
         B = seq_len.numel()
-        self._is(q, "q", torch.float32, (B, self.n_head, self.head_dim))
-        self._is(seq_len, "seq_len", torch.int32)
-        self._is(page_table, "page_table", torch.int32, (B, page_table.shape[-1]))
-        shape = (B, self.n_head * self.head_dim)
-        out = _empty(shape, torch.float32, self._dev, stream) if out is None else self._is(out, "out", torch.float32, shape)
-        lib = _lib.load()
-        d = self._descs[layer]
-        with _on(self._dev):
-            ws = _empty((lib.sfa_decode_window_workspace_bytes(d, B, max_seq_len, window, n_sink),), torch.uint8,
-                        self._dev, stream)
-            _lib.check(lib.sfa_attn_decode_window(
-                d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.shape[1], seq_len.data_ptr(), window,
-                n_sink, B, max_seq_len, self.scale if scale is None else scale, ws.data_ptr(), ws.numel(),
-                _stream(stream)), "sfa_attn_decode_window")
+        out = self._rows(q, out, B, stream)
+        if seq_len.dtype is not i32 or seq_len.get_device() != dev or not seq_len.is_contiguous():
+            raise self._bad("seq_len", "int32", "[B]")
+        if (page_table.dtype is not i32 or page_table.get_device() != dev or page_table.dim() != 2
+                or page_table.shape[0] != B or not page_table.is_contiguous()):
+            raise self._bad("page_table", "int32", f"[{B}, max_pages]")
+        lib, d = _lib.load(), self._descs[layer]
+        key = (B, max_seq_len, window, n_sink)
+        need = self._ws_window.get(key)
+        if need is None:
+            if len(self._ws_window) >= 1024:
+                self._ws_window.clear()
+            need = self._ws_window[key] = lib.sfa_decode_window_workspace_bytes(d, *key)
+        ws = _empty((need,), out, stream, torch.uint8)
+        rc = lib.sfa_attn_decode_window(
+            d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.shape[1], seq_len.data_ptr(), window,
+            n_sink, B, max_seq_len, self._scale if scale is None else scale, ws.data_ptr(), need, _raw_stream(stream, dev))
+        if rc:
+            _lib.check(rc, "sfa_attn_decode_window")
         return out
 
     def prefill_window(self, layer: int, q: torch.Tensor, page_table: torch.Tensor, q_pos0: int, window: int,
@@ -347,17 +383,20 @@ class PagedKV:
         """q [T, Hq, hd] f32 of one sequence -> out [T, Hq*hd] f32: the token at
         position t attends the ``window`` positions up to t and the first
         ``n_sink``.  The workspace is the call's own."""
+        dev = self._index
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.prefill_window(layer, q, page_table, q_pos0, window, n_sink, out, scale, stream)
         T = q.shape[0]
-        self._is(q, "q", torch.float32, (T, self.n_head, self.head_dim))
-        self._is(page_table, "page_table", torch.int32, (page_table.numel(),))
-        shape = (T, self.n_head * self.head_dim)
-        out = _empty(shape, torch.float32, self._dev, stream) if out is None else self._is(out, "out", torch.float32, shape)
-        lib = _lib.load()
-        d = self._descs[layer]
-        with _on(self._dev):
-            need = lib.sfa_prefill_window_workspace_bytes(d, q_pos0, T, window, n_sink)
-            ws = _empty((need,), torch.uint8, self._dev, stream) if need else None
-            _lib.check(lib.sfa_attn_prefill_window(
-                d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.numel(), q_pos0, T, window, n_sink,
-                self.scale if scale is None else scale, _ptr(ws), need, _stream(stream)), "sfa_attn_prefill_window")
+        out = self._rows(q, out, T, stream)
+        if page_table.dtype is not torch.int32 or page_table.get_device() != dev or page_table.dim() != 1 or not page_table.is_contiguous():
+            raise self._bad("page_table", "int32", "[max_pages]")
+        lib, d = _lib.load(), self._descs[layer]
+        need = lib.sfa_prefill_window_workspace_bytes(d, q_pos0, T, window, n_sink)
+        ws = _empty((need,), out, stream, torch.uint8) if need else None
+        rc = lib.sfa_attn_prefill_window(
+            d, q.data_ptr(), out.data_ptr(), page_table.data_ptr(), page_table.shape[0], q_pos0, T, window, n_sink,
+            self._scale if scale is None else scale, _ptr(ws), need, _raw_stream(stream, dev))
+        if rc:
+            _lib.check(rc, "sfa_attn_prefill_window")
         return out
