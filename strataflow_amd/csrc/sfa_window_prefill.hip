@@ -58,7 +58,11 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
     __shared__ __attribute__((aligned(256))) uint8_t lds[BUFS][SETS][T::BYTES];
     __shared__ __attribute__((aligned(16))) float k_scale[kQ8 ? NB : 1][kQ8 ? TP : 4];
     __shared__ int v_exp[4];                 // Q8_0: exponent of each 16 positions' largest V scale
-    __shared__ uint64_t v_bad[4];            // Q8_0: a wave's units whose V scale is not finite, held as zeros
+    // values that are not finite, held as zeros: Q8_0: the units of a wave whose
+    // scale is not; else whether a wave's quarter of the tile has any, and a bit
+    // for each value of a chunk
+    __shared__ uint64_t v_bad[2][4];
+    __shared__ uint8_t v_bits[2][kQ8 ? 4 : TP * T::CPR];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -83,8 +87,9 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
     const int ns = min(min(p.n_sink, lo), hi + 1);
     const int sink_tiles = (ns + TP - 1) / TP;
     const int n_tiles = sink_tiles + (hi >= lo ? hi / TP - lo / TP + 1 : 0);
-    const int t0 = (int)((int64_t)n_tiles * split / p.n_split);
-    const int t1 = (int)((int64_t)n_tiles * (split + 1) / p.n_split);
+    // (the divisions run on the vector side: back to scalars, for scalar branches)
+    const int t0 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * split / p.n_split));
+    const int t1 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * (split + 1) / p.n_split));
 
     PageWindow pages;
     if (t0 < t1)
@@ -159,7 +164,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
         s.first = (s.sink ? t : lo / TP + t - sink_tiles) * TP;
         s.from = max(s.sink ? 0 : lo - s.first, 0);
         s.to = min((s.sink ? ns : hi + 1) - s.first, TP);
-        const int lp = s.first / p.page_size;
+        const int lp = (int)to_scalar((uint32_t)s.first / (uint32_t)p.page_size);
         const int32_t id = pages.get(p.page_table, p.max_pages, lp, lane);
         const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
         const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
                     const float big = wave_max(fabsf(d));
                     const int e = max((int)(__builtin_bit_cast(uint32_t, big) >> 23), 1);
                     if (lane == 0) {
-                        v_bad[wave] = bads;
+                        v_bad[0][wave] = bads;
                         if constexpr (NB == 4) v_exp[wave] = e;
                         else v_exp[2 * (wave - 2)] = v_exp[2 * (wave - 2) + 1] = e;
                     }
@@ -263,6 +268,10 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
     if (t0 < t1) src = issue(t0, 0);
     int buf = 0;
     for (int t = t0; t < t1; ++t, buf ^= BUFS - 1, src = next) {
+        // masked where a row of the workgroup does not see the whole tile
+        const int end = src.first + TP - 1;
+        const bool masked = (src.from > 0) | (src.to < TP) |
+                            (!src.sink & ((end > first) | ((src.first <= last - p.window) & (end >= p.n_sink))));
         if constexpr (kQ8) {
             __syncthreads();  // the last tile has been read
             stage();
@@ -270,6 +279,35 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
             __syncthreads();
         } else {
             wait_loads<0>();
+            // a value that is not finite would reach rows that do not see it, as
+            // 0 times it: the wave looks its quarter of V over
+            if (masked) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < T::NI; ++i) {
+                    const int ch = (T::NI * wave + i) * 64 + lane;
+                    intx4 *const at = reinterpret_cast<intx4 *>(&lds[buf][1][16 * ch]);
+                    intx4 x = *at;
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int j = 0; j < (kF32 ? 4 : 8); ++j) {
+                        const uint32_t e = kF32 ? (uint32_t)x[j & 3] >> 23 & 255 : (uint32_t)x[j / 2] >> (j % 2 ? 26 : 10) & 31;
+                        bits |= (e == (kF32 ? 255u : 31u) ? 1u : 0u) << j;
+                    }
+                    if (bits != 0) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (kF32) x[j] = bits >> j & 1 ? 0 : x[j];
+                            else x[j] &= (bits >> 2 * j & 1 ? 0 : 0xffff) | (bits >> (2 * j + 1) & 1 ? 0 : (int)0xffff0000);
+                        }
+                        *at = x;
+                        any = true;
+                    }
+                    v_bits[buf][ch] = (uint8_t)bits;
+                }
+                const uint64_t who = __ballot(any);
+                if (lane == 0) v_bad[buf][wave] = who;
+            }
             __syncthreads();  // this tile is there, and the other buffer has been read
             if (t + 1 < t1) next = issue(t + 1, buf ^ 1);
         }
@@ -323,14 +361,11 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
                 }
         }
 
-        // masked where a row of the workgroup does not see the whole tile
-        const int end = src.first + TP - 1;
-        const bool masked = src.from > 0 || src.to < TP || (!src.sink && (end > first || (src.first <= last - p.window && end >= p.n_sink)));
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 16 * PB; ++i) {
                 const int r = i / 16 * 32 + i / 4 % 4 * 8 + 4 * hh + i % 4, pos = src.first + r;
-                const bool see = r >= src.from && r < src.to && pos <= tpos && (src.sink || pos > tpos - p.window || pos < p.n_sink);
+                const bool see = (r >= src.from) & (r < src.to) & (pos <= tpos) & (src.sink | (pos > tpos - p.window) | (pos < p.n_sink));
                 s[i / 16][i % 16] = see ? s[i / 16][i % 16] : -INFINITY;
             }
         }
@@ -364,12 +399,12 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
         auto spoil = [&]() {
             for (int r = src.from; r < src.to; ++r) {
                 const int pos = src.first + r;
-                const bool see = pos <= tpos && (src.sink || pos > tpos - p.window || pos < p.n_sink);
+                const bool see = (pos <= tpos) & (src.sink | (pos > tpos - p.window) | (pos < p.n_sink));
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     if constexpr (kQ8) {
                         const int u = r * NB + d;  // its unit, NB / 2 * 128 of them in the waves that hold V
-                        const bool bad = v_bad[(NB == 4 ? 0 : 2) + u / 64] >> u % 64 & 1;
+                        const bool bad = v_bad[0][(NB == 4 ? 0 : 2) + u / 64] >> u % 64 & 1;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[d][i] = bad && see ? NAN : o[d][i];
                         continue;
@@ -377,10 +412,9 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int e = 32 * d + i / 4 * 8 + 4 * hh + i % 4;  // the dim of o[d][i]
-                        float v;
-                        if constexpr (kF32) v = *reinterpret_cast<const float *>(vt + r * T::ROW + 16 * pv_slot<KVT, HD>(r, e / 4) + 4 * (e % 4));
-                        else v = (float)*reinterpret_cast<const _Float16 *>(vt + r * T::ROW + 16 * pv_slot<KVT, HD>(r, e / 8) + 2 * (e % 8));
-                        if (see) o[d][i] += v - v;
+                        constexpr int PC = kF32 ? 4 : 8;                    // values of a chunk
+                        const bool bad = v_bits[buf][r * T::CPR + pv_slot<KVT, HD>(r, e / PC)] >> e % PC & 1;
+                        o[d][i] = (bad & see) ? NAN : o[d][i];
                     }
                 }
             }
@@ -390,25 +424,10 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
                 const int r = i / 4 * 8 + 4 * hh + i % 4;
                 return *reinterpret_cast<const float *>(vt + r * T::ROW + 16 * pv_slot<KVT, HD>(r, 8 * d + n / 4) + 4 * (n & 3));
             };
-            if (masked) {
-                bool odd = false;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        float a = v_at(i, d);
-                        const bool bad = !(fabsf(a) < INFINITY);
-                        odd |= bad;
-                        a = bad ? 0.0f : a;
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][i], o[d], 0, 0, 0);
-                    }
-                if (__ballot(odd) != 0) spoil();
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v_at(i, d), s[0][i], o[d], 0, 0, 0);
-            }
+                for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v_at(i, d), s[0][i], o[d], 0, 0, 0);
         } else {
             constexpr int ST = TP / 16;  // 16-position steps
             float w16[ST];
@@ -446,43 +465,23 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
                 const half4 y = tr16_read(tile + rb * T::ROW + 16 * pv_slot<KVT, HD>(rb, ch) + sub8);
                 return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             };
-            if (!kQ8 && masked) {
-                uint32_t odd = 0;
 #pragma unroll
-                for (int st = 0; st < ST; ++st)
+            for (int st = 0; st < ST; ++st)
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        intx4 a = __builtin_bit_cast(intx4, v_at(vt, st, d));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            // bit 15 of a half whose exponent is all ones: 0x7c00 + 0x0400
-                            const uint32_t bad = ((a[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                            odd |= bad;
-                            a[j] &= ~((bad >> 15) * 0xffffu);
-                        }
-                        const half8 v = __builtin_bit_cast(half8, a);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[st], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[st], o[d], 0, 0, 0);
+                for (int d = 0; d < DB; ++d) {
+                    const half8 a = v_at(vt, st, d);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
+                    if constexpr (kQ8) {
+                        const half8 b = v_at(lds[0][SETS - 1], st, d);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[st], o[d], 0, 0, 0);
                     }
-                if (__ballot(odd != 0) != 0) spoil();
-            } else {
-#pragma unroll
-                for (int st = 0; st < ST; ++st)
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const half8 a = v_at(vt, st, d);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
-                        if constexpr (kQ8) {
-                            const half8 b = v_at(lds[0][SETS - 1], st, d);
-                            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[st], o[d], 0, 0, 0);
-                        }
-                    }
-                if constexpr (kQ8) {
-                    const uint64_t any = NB == 4 ? v_bad[0] | v_bad[1] | v_bad[2] | v_bad[3] : v_bad[2] | v_bad[3];
-                    if (__ballot(any != 0) != 0) spoil();
                 }
-            }
+        }
+        if (kQ8 || masked) {
+            const uint64_t *const vb = v_bad[buf];
+            const uint64_t any = kQ8 && NB == 2 ? vb[2] | vb[3] : vb[0] | vb[1] | vb[2] | vb[3];
+            if (__ballot(any != 0) != 0) spoil();
         }
     }
     if (!row_ok) return;
