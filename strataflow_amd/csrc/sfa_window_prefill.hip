@@ -45,6 +45,25 @@ __device__ inline int pv_slot(int r, int j) {
     return j ^ (r / T::RP % T::NG * 4);
 }
 
+// Runs the N steps of a product loop with the operand reads AHEAD steps before
+// their use; left to itself the compiler waits for every operand right before
+// it is used.  Vector and scalar arithmetic may move over the fences, reads and
+// matrix instructions may not.
+template <int N, int AHEAD, typename Read, typename Use>
+__device__ inline void pipelined(Read read, Use use) {
+    decltype(read(0)) a[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < N; ++i) a[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const auto now = a[i % AHEAD];
+        if (i + AHEAD < N) a[i % AHEAD] = read(i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0x406);
+        use(i, now);
+        __builtin_amdgcn_sched_barrier(0x406);
+    }
+}
+
 template <int KVT, int HD, int G>
 __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) {
     using T = PTile<KVT, HD>;
@@ -313,6 +332,18 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
         }
         if (!wave_ok || !src.there) continue;
         const uint8_t *const kt = lds[kQ8 ? 0 : buf][0], *const vt = lds[kQ8 ? 0 : buf][1];
+        // This lane's first operand addresses; a step's are these with its chunk
+        // XORed in (the slots are XORs too) and its rows added.  The empty asm
+        // keeps the compiler from holding every step's address over the loop.
+        int k_at = n * T::ROW + 16 * pk_slot<KVT, HD>(n, hh), v_at0 = 0;
+        const int li = lane & 15;
+        if constexpr (kF32) {
+            v_at0 = 4 * hh * T::ROW + 16 * pv_slot<KVT, HD>(4 * hh, n / 4) + 4 * (n & 3);
+        } else {
+            const int r = 4 * hh + (li >> 2);
+            v_at0 = r * T::ROW + 16 * pv_slot<KVT, HD>(r, 2 * (lane >> 4 & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
+        }
+        asm("" : "+v"(k_at), "+v"(v_at0));
 
         floatx16 s[PB];
 #pragma unroll
@@ -320,45 +351,45 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
         if constexpr (kF32) {
+            pipelined<2 * KC, 3>([&](int c) { return *reinterpret_cast<const floatx4 *>(kt + (k_at ^ (32 * c))); },
+                                 [&](int c, floatx4 a) {
 #pragma unroll
-            for (int c = 0; c < 2 * KC; ++c) {
-                const floatx4 a = *reinterpret_cast<const floatx4 *>(kt + n * T::ROW + 16 * pk_slot<KVT, HD>(n, 2 * c + hh));
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], qf[c / 2][c % 2 * 4 + i], s[0], 0, 0, 0);
-            }
+                                     for (int i = 0; i < 4; ++i)
+                                         s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], qf[c / 2][c % 2 * 4 + i], s[0], 0, 0, 0);
+                                 });
         } else if constexpr (!kQ8) {
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int b = 0; b < PB; ++b) {
-                    const int r = 32 * b + n;
-                    const half8 a = *reinterpret_cast<const half8 *>(kt + r * T::ROW + 16 * pk_slot<KVT, HD>(r, 2 * c + hh));
+            pipelined<KC * PB, 3>(
+                [&](int i) {
+                    return *reinterpret_cast<const half8 *>(kt + (k_at ^ (32 * (i / PB))) + i % PB * 32 * T::ROW);
+                },
+                [&](int i, half8 a) {
+                    const int c = i / PB, b = i % PB;
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], s[b], 0, 0, 0);
                     s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], s[b], 0, 0, 0);
-                }
+                });
         } else {
+            // two steps a block, then the block's scales
+            floatx16 x;
+            pipelined<KC * PB, 3>(
+                [&](int i) {
+                    const int b = i / 2 % PB, c = i / (2 * PB) * 2 + i % 2;
+                    return *reinterpret_cast<const half8 *>(kt + (k_at ^ (32 * c)) + b * 32 * T::ROW);
+                },
+                [&](int i, half8 a) {
+                    const int b = i / 2 % PB, nb = i / (2 * PB), c = 2 * nb + i % 2;
+                    if (i % 2 == 0)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int b = 0; b < PB; ++b) {
-                    const int r = 32 * b + n;
-                    floatx16 x;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-#pragma unroll
-                    for (int c = 2 * nb; c < 2 * nb + 2; ++c) {
-                        const half8 a = *reinterpret_cast<const half8 *>(kt + r * T::ROW + 16 * pk_slot<KVT, HD>(r, 2 * c + hh));
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], x, 0, 0, 0);
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], x, 0, 0, 0);
-                    }
+                        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], x, 0, 0, 0);
+                    if (i % 2 == 0) return;
 #pragma unroll
                     for (int i4 = 0; i4 < 4; ++i4) {
                         const floatx4 d = *reinterpret_cast<const floatx4 *>(&k_scale[nb][32 * b + 8 * i4 + 4 * hh]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[b][4 * i4 + i] = fmaf(x[4 * i4 + i], d[i], s[b][4 * i4 + i]);
+                        for (int j = 0; j < 4; ++j) s[b][4 * i4 + j] = fmaf(x[4 * i4 + j], d[j], s[b][4 * i4 + j]);
                     }
-                }
+                });
         }
 
         if (masked) {
@@ -420,14 +451,10 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
             }
         };
         if constexpr (kF32) {
-            auto v_at = [&](int i, int d) {
-                const int r = i / 4 * 8 + 4 * hh + i % 4;
-                return *reinterpret_cast<const float *>(vt + r * T::ROW + 16 * pv_slot<KVT, HD>(r, 8 * d + n / 4) + 4 * (n & 3));
-            };
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v_at(i, d), s[0][i], o[d], 0, 0, 0);
+            // rows 8 (i / 4) + 4 hh + i % 4: the slots of all are those of row 4 hh
+            pipelined<16 * DB, 4>(
+                [&](int i) { return *reinterpret_cast<const float *>(vt + (v_at0 ^ (128 * (i % DB))) + (i / DB / 4 * 8 + i / DB % 4) * T::ROW); },
+                [&](int i, float a) { o[i % DB] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][i / DB], o[i % DB], 0, 0, 0); });
         } else {
             constexpr int ST = TP / 16;  // 16-position steps
             float w16[ST];
@@ -457,26 +484,21 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
                 }
             // operand of step st: positions 16 st + 4 hh .. and 16 st + 8 + 4 hh .., the lane's own
             // scores; four values a read, lane i of 16 gets dim i of the four rows its group names
-            const int li = lane & 15, dsub = lane >> 4 & 1;
             auto v_at = [&](const uint8_t *tile, int st, int d) {
-                const int ra = 16 * st + 4 * hh + (li >> 2), rb = ra + 8;
-                const int ch = 4 * d + 2 * dsub + ((li & 3) >> 1), sub8 = 8 * (li & 1);
-                const half4 x = tr16_read(tile + ra * T::ROW + 16 * pv_slot<KVT, HD>(ra, ch) + sub8);
-                const half4 y = tr16_read(tile + rb * T::ROW + 16 * pv_slot<KVT, HD>(rb, ch) + sub8);
+                const uint8_t *const at = tile + (v_at0 ^ (64 * d)) + 16 * st * T::ROW;
+                const half4 x = tr16_read(at), y = tr16_read(at + 8 * T::ROW);
                 return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             };
-#pragma unroll
-            for (int st = 0; st < ST; ++st)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const half8 a = v_at(vt, st, d);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
-                    if constexpr (kQ8) {
-                        const half8 b = v_at(lds[0][SETS - 1], st, d);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[st], o[d], 0, 0, 0);
-                    }
-                }
+            pipelined<ST * DB, 3>([&](int i) { return v_at(vt, i / DB, i % DB); },
+                                  [&](int i, half8 a) {
+                                      const int st = i / DB, d = i % DB;
+                                      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
+                                      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
+                                      if constexpr (kQ8) {
+                                          const half8 b = v_at(lds[0][SETS - 1], st, d);
+                                          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[st], o[d], 0, 0, 0);
+                                      }
+                                  });
         }
         if (kQ8 || masked) {
             const uint64_t *const vb = v_bad[buf];
