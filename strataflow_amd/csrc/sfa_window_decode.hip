@@ -50,21 +50,6 @@ __device__ inline int v_slot(int r, int j) {
     return j;
 }
 
-// 8 quants at a 2-byte aligned LDS address as f16 (exact): byte b is 1024 +
-// (b + 128) under the exponent of 1024.
-__device__ inline half2v quants2(uint32_t two) {  // bytes 0 and 2
-    const half2v base = {(_Float16)1152.0f, (_Float16)1152.0f};
-    return __builtin_bit_cast(half2v, two ^ 0x64806480u) - base;
-}
-__device__ inline half8 quants8(uint32_t a, uint32_t b) {
-    half8 r;
-    const half2v h[4] = {quants2(__builtin_amdgcn_perm(0, a, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, a, 0x0c030c02)),
-                         quants2(__builtin_amdgcn_perm(0, b, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, b, 0x0c030c02))};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[2 * i] = h[i][0], r[2 * i + 1] = h[i][1];
-    return r;
-}
-
 template <int KVT, int HD, int G>
 __global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowParams p) {
     using T = Tile<KVT, HD>;

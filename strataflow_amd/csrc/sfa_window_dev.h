@@ -117,6 +117,15 @@ __device__ inline void split_f16(float x, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
+// Two values split so, in four instructions: what is left of x is h (-1) + x as
+// a dot product with the pair, exact (the other half meets a zero).
+__device__ inline void split2_f16(float x, float y, half2v &hi, half2v &lo) {
+    const half2v h = {(_Float16)x, (_Float16)y};
+    const half2v first = {(_Float16)-1.0f, (_Float16)0.0f}, second = {(_Float16)0.0f, (_Float16)-1.0f};
+    hi = h;
+    lo = half2v{(_Float16)__builtin_amdgcn_fdot2(h, first, x, false), (_Float16)__builtin_amdgcn_fdot2(h, second, y, false)};
+}
+
 // Power of two that takes a row's largest value into [2^14, 2^15), and its
 // inverse.
 __device__ inline void row_exponent(float amax, float &down, float &up) {
@@ -124,6 +133,20 @@ __device__ inline void row_exponent(float amax, float &down, float &up) {
     e = e < kSplitShift + 2 ? kSplitShift + 2 : e > 252 ? 252 : e;  // zeros and the ends of the range
     down = __builtin_bit_cast(float, (uint32_t)(254 + kSplitShift - e) << 23);
     up = __builtin_bit_cast(float, (uint32_t)(e - kSplitShift) << 23);
+}
+
+// Quants as f16 (exact): byte b is 1024 + (b + 128) under the exponent of 1024.
+__device__ inline half2v quants2(uint32_t two) {  // bytes 0 and 2
+    const half2v base = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(half2v, two ^ 0x64806480u) - base;
+}
+__device__ inline half8 quants8(uint32_t a, uint32_t b) {
+    half8 r;
+    const half2v h[4] = {quants2(__builtin_amdgcn_perm(0, a, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, a, 0x0c030c02)),
+                         quants2(__builtin_amdgcn_perm(0, b, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, b, 0x0c030c02))};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[2 * i] = h[i][0], r[2 * i + 1] = h[i][1];
+    return r;
 }
 
 }  // namespace sfa

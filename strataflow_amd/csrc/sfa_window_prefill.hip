@@ -13,6 +13,8 @@
 //
 // Chunks of few rows leave CUs idle: their tiles are split over workgroups,
 // whose records window_merge_kernel joins.
+#include <type_traits>
+
 #include "sfa_window_dev.h"
 
 namespace sfa {
@@ -21,27 +23,26 @@ constexpr int kRows = 128;  // of a workgroup
 
 template <int KVT, int HD>
 struct PTile {
-    static constexpr int TP = KVT == SFA_KV_F32 ? 32 : 64;           // positions
-    static constexpr int ROW = KVT == SFA_KV_F32 ? HD * 4 : HD * 2;  // a row in LDS (Q8_0: its quants as f16)
-    static constexpr int RB = KVT == SFA_KV_Q8_0 ? HD / kQK * kQ8Bytes : ROW;
+    static constexpr int TP = KVT == SFA_KV_F32 ? 32 : 64;  // positions
+    static constexpr int RB = KVT == SFA_KV_F32 ? HD * 4 : KVT == SFA_KV_F16 ? HD * 2 : HD / kQK * kQ8Bytes;
+    static constexpr int ROW = HD * 2;                      // a row in LDS: f16, or f16 halves of wider values
     static constexpr int CPR = ROW / 16;
     static constexpr int BYTES = TP * ROW;
-    static constexpr int NI = BYTES / 4096;  // load instructions of a wave, a tensor
+    static constexpr int NI = BYTES / 4096;                 // F16: load instructions of a wave, a tensor
     static constexpr int RP = 256 / ROW > 0 ? 256 / ROW : 1;  // rows under all LDS banks
     static constexpr int NG = ROW / 64 > 0 ? ROW / 64 : 1;
 };
 
 // Where chunk j of row r lies in its LDS row: K's reads are 16 rows at one
-// chunk, V's four rows at 64 neighbouring bytes (F32: two rows at 128).
-template <int KVT, int HD>
+// chunk, V's four rows at 64 neighbouring bytes.
+template <int HD>
 __device__ inline int pk_slot(int r, int j) {
-    using T = PTile<KVT, HD>;
-    return j ^ (r / T::RP % (T::CPR < 16 ? T::CPR : 16));
+    using T = PTile<SFA_KV_F16, HD>;
+    return j ^ (r / T::RP % T::CPR);
 }
-template <int KVT, int HD>
+template <int HD>
 __device__ inline int pv_slot(int r, int j) {
-    using T = PTile<KVT, HD>;
-    if constexpr (KVT == SFA_KV_F32) return j ^ (r / 4 % 2 * (T::CPR >= 16 ? 8 : 0));
+    using T = PTile<SFA_KV_F16, HD>;
     return j ^ (r / T::RP % T::NG * 4);
 }
 
@@ -49,7 +50,7 @@ __device__ inline int pv_slot(int r, int j) {
 // their use; left to itself the compiler waits for every operand right before
 // it is used.  Vector and scalar arithmetic may move over the fences, reads and
 // matrix instructions may not.
-template <int N, int AHEAD, typename Read, typename Use>
+template <int N, int AHEAD, int FENCE = 0x406, typename Read, typename Use>
 __device__ inline void pipelined(Read read, Use use) {
     decltype(read(0)) a[AHEAD];
 #pragma unroll
@@ -58,355 +59,281 @@ __device__ inline void pipelined(Read read, Use use) {
     for (int i = 0; i < N; ++i) {
         const auto now = a[i % AHEAD];
         if (i + AHEAD < N) a[i % AHEAD] = read(i + AHEAD);
-        __builtin_amdgcn_sched_barrier(0x406);
+        __builtin_amdgcn_sched_barrier(FENCE);
         use(i, now);
-        __builtin_amdgcn_sched_barrier(0x406);
+        __builtin_amdgcn_sched_barrier(FENCE);
     }
 }
 
-template <int KVT, int HD, int G>
-__global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) {
-    using T = PTile<KVT, HD>;
-    constexpr int TP = T::TP, PB = TP / 32;  // 32-position blocks of a tile
-    constexpr int DB = HD / 32;
-    constexpr int KC = HD / 16;              // 16-dim steps of a score (F32: pairs of 4-float chunks are 2 KC)
-    constexpr int NB = HD / kQK;
-    constexpr bool kQ8 = KVT == SFA_KV_Q8_0, kF32 = KVT == SFA_KV_F32;
-    constexpr int BUFS = kQ8 ? 1 : 2;        // Q8_0 tiles wait in registers
-    constexpr int SETS = kQ8 ? 3 : 2;        // K, V; Q8_0: K, V's two halves
-    __shared__ __attribute__((aligned(256))) uint8_t lds[BUFS][SETS][T::BYTES];
-    __shared__ __attribute__((aligned(16))) float k_scale[kQ8 ? NB : 1][kQ8 ? TP : 4];
-    __shared__ int v_exp[4];                 // Q8_0: exponent of each 16 positions' largest V scale
-    // values that are not finite, held as zeros: Q8_0: the units of a wave whose
-    // scale is not; else whether a wave's quarter of the tile has any, and a bit
-    // for each value of a chunk
-    __shared__ uint64_t v_bad[2][4];
-    __shared__ uint8_t v_bits[2][kQ8 ? 4 : TP * T::CPR];
+// A lane's row, and its workgroup's rows and tiles.
+struct Block {
+    int kvh, split;
+    int tok, head, tpos;   // the lane's row: its token (a row past the chunk: the last), head and position
+    bool row_ok, wave_ok;  // the lane has a row, the wave has any
+    int first, last;       // positions of the workgroup's tokens
+    int lo, hi, ns;        // what any of them sees: sinks before the window [0, ns), then [lo, hi]
+    int sink_tiles, t0, t1;
+};
+template <int G, int TP>
+__device__ inline Block block_of(const WindowParams &p, int wave, int n) {
+    Block b;
+    // Workgroups go round the eight XCDs: with Hkv a multiple of 8 a kv head's
+    // tiles stay in one L2.  The last rows, which see the most, come first.
+    const int blk = gridDim.z - 1 - blockIdx.z;
+    b.kvh = blockIdx.x;
+    b.split = blockIdx.y;
+    const int row = blk * kRows + wave * 32 + n;  // token row / G, head row % G of the group
+    b.row_ok = row < p.n_tok * G;
+    b.tok = b.row_ok ? row / G : p.n_tok - 1;
+    b.head = b.kvh * G + row % G;
+    b.tpos = p.q_pos0 + b.tok;
+    b.wave_ok = blk * kRows + wave * 32 < p.n_tok * G;
+    const int64_t cap = (int64_t)p.max_pages * p.page_size;
+    b.first = p.q_pos0 + blk * kRows / G;
+    b.last = p.q_pos0 + min((blk * kRows + kRows - 1) / G, p.n_tok - 1);
+    b.lo = b.first - p.window + 1 > 0 ? b.first - p.window + 1 : 0;
+    b.hi = b.last < cap ? b.last : (int)(cap - 1);
+    b.ns = min(min(p.n_sink, b.lo), b.hi + 1);
+    b.sink_tiles = (b.ns + TP - 1) / TP;
+    const int n_tiles = b.sink_tiles + (b.hi >= b.lo ? b.hi / TP - b.lo / TP + 1 : 0);
+    // (the divisions run on the vector side: back to scalars, for scalar branches)
+    b.t0 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * b.split / p.n_split));
+    b.t1 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * (b.split + 1) / p.n_split));
+    return b;
+}
 
+// A tile: where it lies and which of its rows any token of the workgroup sees.
+struct Src {
+    int first, from, to;       // position of its row 0, its visible rows
+    bool sink, there, masked;  // masked: some row of the workgroup does not see all of it
+    const uint8_t *k, *v;      // its first visible rows
+    int bytes, back;           // of the visible rows; offset of the first from row 0
+};
+template <int TP, int RB>
+__device__ inline Src source(const WindowParams &p, const Block &b, PageWindow &pages, int t, int lane) {
+    const int col_bytes = p.n_head_kv * RB;
+    Src s;
+    s.sink = t < b.sink_tiles;
+    s.first = (s.sink ? t : b.lo / TP + t - b.sink_tiles) * TP;
+    s.from = max(s.sink ? 0 : b.lo - s.first, 0);
+    s.to = min((s.sink ? b.ns : b.hi + 1) - s.first, TP);
+    const int lp = (int)to_scalar((uint32_t)s.first / (uint32_t)p.page_size);
+    const int32_t id = pages.get(p.page_table, p.max_pages, lp, lane);
+    const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
+    const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
+    s.there = kb != nullptr && vb != nullptr;
+    const int64_t at = (int64_t)(s.first - lp * p.page_size + s.from) * col_bytes + b.kvh * RB;
+    s.k = s.there ? kb + at : nullptr;
+    s.v = s.there ? vb + at : nullptr;
+    s.bytes = s.there ? (s.to - s.from - 1) * col_bytes + RB : 0;
+    s.back = s.from * col_bytes;
+    const int end = s.first + TP - 1;
+    s.masked = (s.from > 0) | (s.to < TP) | !s.there |
+               (!s.sink & ((end > b.first) | ((s.first <= b.last - p.window) & (end >= p.n_sink))));
+    return s;
+}
+template <int TP>
+__device__ inline void page_window(const WindowParams &p, const Block &b, PageWindow &pages, int lane) {
+    const int t = b.t0;
+    if (t < b.t1)
+        pages.load(p.page_table, p.max_pages, (t < b.sink_tiles ? t : b.lo / TP + t - b.sink_tiles) * TP / p.page_size, lane);
+}
+
+// Whether the token at tpos sees row r of a tile.
+__device__ inline bool sees(const WindowParams &p, const Src &s, int r, int tpos) {
+    const int pos = s.first + r;
+    return (r >= s.from) & (r < s.to) & (pos <= tpos) & (s.sink | (pos > tpos - p.window) | (pos < p.n_sink)) & s.there;
+}
+
+// A value of V that is not finite would reach rows that do not see it, as 0
+// times it.  Each wave looks its quarter of a masked tile over: such values
+// become zeros and get a bit, and the rows that see one are NaN afterwards.
+template <int HD>
+__device__ inline void look_over(uint8_t *v, uint8_t *bits_of, uint64_t *bad, int wave, int lane) {
+    using T = PTile<SFA_KV_F16, HD>;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) {
+        const int ch = (T::NI * wave + i) * 64 + lane;
+        intx4 *const at = reinterpret_cast<intx4 *>(v + 16 * ch);
+        intx4 x = *at;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bits |= (((uint32_t)x[j / 2] >> (j % 2 ? 26 : 10) & 31) == 31 ? 1u : 0u) << j;
+        if (bits != 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] &= (bits >> 2 * j & 1 ? 0 : 0xffff) | (bits >> (2 * j + 1) & 1 ? 0 : (int)0xffff0000);
+            *at = x;
+            any = true;
+        }
+        bits_of[ch] = (uint8_t)bits;
+    }
+    const uint64_t who = __ballot(any);
+    if (lane == 0) bad[wave] = who;
+}
+
+__device__ inline bool any_bad(const uint64_t *bad) { return __ballot((bad[0] | bad[1] | bad[2] | bad[3]) != 0) != 0; }
+
+// NaN to the outputs of the lane's row that a value set to zero has a part in;
+// was(r, e): whether V's value e of row r was.
+template <int HD, typename O, typename Was>
+__device__ inline void spoil(const WindowParams &p, const Src &s, int tpos, int hh, O &o, Was was) {
+    asm("" : "+v"(hh));  // (its 16 multiples are not held over the loop)
+    for (int r = s.from; r < s.to; ++r) {
+        const bool see = sees(p, s, r, tpos);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = 32 * d + i / 4 * 8 + 4 * hh + i % 4;  // the dim of o[d][i]
+                o[d][i] = (was(r, e) & see) ? NAN : o[d][i];
+                if (i % 4 == 3) asm volatile("" ::: "memory");  // few reads at a time
+            }
+    }
+}
+
+// The lane's outputs, or its split record.
+template <int HD, typename O>
+__device__ inline void store_row(const WindowParams &p, const Block &b, int hh, const O &o, float base, float l, float unit) {
+    if (!b.row_ok) return;
+    float la, lb;
+    swap_halves(l, la, lb);
+    l = la + lb;
+    const float w = p.n_split > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
+    const int64_t row = (int64_t)b.tok * p.n_head + b.head;
+    float *const dst = p.n_split > 1 ? p.rec_o + (row * p.n_split + b.split) * HD : p.out + row * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            floatx4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = o[d][4 * i4 + i] * w;
+            *reinterpret_cast<floatx4 *>(dst + 32 * d + 8 * i4 + 4 * hh) = x;
+        }
+    if (p.n_split > 1 && hh == 0) p.rec_ml[row * p.n_split + b.split] = make_float2(base, l);
+}
+
+// Q of a lane's row, dims 16 c + 8 hh + j, as two f16 under a power of two of
+// the row; returns that power's inverse.
+template <int HD>
+__device__ inline float split_q(const float *q, half8 (&qh)[HD / 16], half8 (&ql)[HD / 16]) {
+    float x[HD / 16][8], amax = 0.0f, a, b, down, up;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+        const floatx4 u = *reinterpret_cast<const floatx4 *>(q + 16 * c);
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(q + 16 * c + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[c][j] = u[j], x[c][4 + j] = v[j];
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[c][j]));
+    swap_halves(amax, a, b);
+    row_exponent(fmaxf(a, b), down, up);
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            half2v h, l;
+            split2_f16(x[c][j] * down, x[c][j + 1] * down, h, l);
+            qh[c][j] = h[0], qh[c][j + 1] = h[1];
+            ql[c][j] = l[0], ql[c][j + 1] = l[1];
+        }
+    return up;
+}
+
+// The F16 kernel.
+template <int HD, int G>
+__global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams p) {
+    using T = PTile<SFA_KV_F16, HD>;
+    constexpr int TP = T::TP, PB = TP / 32, DB = HD / 32, KC = HD / 16, ST = TP / 16;
+    __shared__ __attribute__((aligned(256))) uint8_t lds[4][T::BYTES];  // K, K, V, V
+    __shared__ uint64_t v_bad[2][4];  // (two of each: a slow wave may still read the last tile's)
+    __shared__ uint8_t v_bits[2][TP * T::CPR];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hh = lane >> 5;
-    // Workgroups go round the eight XCDs: with Hkv a multiple of 8 a kv head's
-    // tiles stay in one L2.  The last rows, which see the most, come first.
-    const int kvh = blockIdx.x, split = blockIdx.y, blk = gridDim.z - 1 - blockIdx.z;
-
-    const int row = blk * kRows + wave * 32 + n;  // token row / G, head row % G of the group
-    const bool row_ok = row < p.n_tok * G;
-    const int tok = row_ok ? row / G : p.n_tok - 1;
-    const int head = kvh * G + row % G;
-    const int tpos = p.q_pos0 + tok;
-    const bool wave_ok = blk * kRows + wave * 32 < p.n_tok * G;
-
-    // the workgroup's span: sinks before the window [0, ns), then [lo, hi]
-    const int tok0 = blk * kRows / G, tok1 = min((blk * kRows + kRows - 1) / G, p.n_tok - 1);
-    const int64_t cap = (int64_t)p.max_pages * p.page_size;
-    const int first = p.q_pos0 + tok0, last = p.q_pos0 + tok1;
-    const int lo = first - p.window + 1 > 0 ? first - p.window + 1 : 0;
-    const int hi = last < cap ? last : (int)(cap - 1);
-    const int ns = min(min(p.n_sink, lo), hi + 1);
-    const int sink_tiles = (ns + TP - 1) / TP;
-    const int n_tiles = sink_tiles + (hi >= lo ? hi / TP - lo / TP + 1 : 0);
-    // (the divisions run on the vector side: back to scalars, for scalar branches)
-    const int t0 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * split / p.n_split));
-    const int t1 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * (split + 1) / p.n_split));
-
+    const Block b = block_of<G, TP>(p, wave, n);
     PageWindow pages;
-    if (t0 < t1)
-        pages.load(p.page_table, p.max_pages, (t0 < sink_tiles ? t0 : lo / TP + t0 - sink_tiles) * TP / p.page_size, lane);
+    page_window<TP>(p, b, pages, lane);
 
-    // Q of this lane's row: dims 16 c + 8 hh + j (F32: 16 c + 4 hh + j and 16 c + 8 + 4 hh + j)
-    const float *const qr = p.q + ((int64_t)tok * p.n_head + head) * HD;
-    float up = 1.0f;
-    half8 qh[kF32 ? 1 : KC], ql[kF32 ? 1 : KC];
-    float qf[kF32 ? KC : 1][8];
-    {
-        float qx[KC][8];
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int d0 = kF32 ? 16 * c + 4 * hh : 16 * c + 8 * hh, d1 = kF32 ? d0 + 8 : d0 + 4;
-            const floatx4 u = *reinterpret_cast<const floatx4 *>(qr + d0);
-            const floatx4 v = *reinterpret_cast<const floatx4 *>(qr + d1);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) qx[c][j] = u[j], qx[c][4 + j] = v[j];
-        }
-        if constexpr (kF32) {
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) qf[c][j] = qx[c][j];
-        } else {
-            float amax = 0.0f, a, b, down;
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(qx[c][j]));
-            swap_halves(amax, a, b);
-            row_exponent(fmaxf(a, b), down, up);
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    _Float16 h, l;
-                    split_f16(qx[c][j] * down, h, l);
-                    qh[c][j] = h;
-                    ql[c][j] = l;
-                }
-        }
-    }
-    const float f = p.scale_log2 * up;
+    half8 qh[KC], ql[KC];
+    const float f = p.scale_log2 * split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql);
 
+    // This wave's quarter of a tile, lane by lane: load i has RPI rows more than
+    // load 0, which flips bit 2 of K's slots i times and leaves V's (few registers:
+    // what the compiler cannot hold it would reload behind the tile's loads).
+    constexpr int RPI = 64 / T::CPR;
+    static_assert(RPI % (4 * T::RP) == 0 || T::NI == 1, "the slots of load i");
     const int col_bytes = p.n_head_kv * T::RB;
-    // F16 and F32: this wave's quarter of a tile, lane by lane
-    int k_off[T::NI], v_off[T::NI];
-    if constexpr (!kQ8) {
+    const int r_0 = T::NI * RPI * wave + lane / T::CPR;
+    const int row_off = r_0 * col_bytes;
+    const int k_chunk = 16 * pk_slot<HD>(r_0, lane % T::CPR), v_chunk = 16 * pv_slot<HD>(r_0, lane % T::CPR);
+    const uint32_t my_lds = lds_addr(lds[0]) + 1024 * T::NI * wave;
+    auto load_k = [&](const Src &s, int buf) {
+        const auto r = buffer_of(s.k, s.bytes);
 #pragma unroll
-        for (int i = 0; i < T::NI; ++i) {
-            const int ch = (T::NI * wave + i) * 64 + lane, r = ch / T::CPR, j = ch % T::CPR;
-            k_off[i] = r * col_bytes + 16 * pk_slot<KVT, HD>(r, j);
-            v_off[i] = r * col_bytes + 16 * pv_slot<KVT, HD>(r, j);
-        }
-    }
-    // Q8_0: units of one block; with HD 128 a thread has one of K and one of V,
-    // with HD 64 the first two waves have K's and the others V's
-    constexpr int UN = kQ8 ? NB / 2 : 1;
-    const int unit = NB == 4 ? threadIdx.x : threadIdx.x & 127;
-    const int u_row = unit / NB, u_blk = unit % NB;
-    uint32_t raw[UN][9];
-
-    struct Src {
-        int first, from, to;  // position of the tile's row 0, and the rows that any token sees
-        bool sink, there;
+        for (int i = 0; i < T::NI; ++i)
+            load_to_lds(r, my_lds + buf * T::BYTES + 1024 * i, row_off + (i * RPI * col_bytes - s.back) + (k_chunk ^ (64 * i)));
     };
-    auto issue = [&](int t, int buf) {
-        Src s;
-        s.sink = t < sink_tiles;
-        s.first = (s.sink ? t : lo / TP + t - sink_tiles) * TP;
-        s.from = max(s.sink ? 0 : lo - s.first, 0);
-        s.to = min((s.sink ? ns : hi + 1) - s.first, TP);
-        const int lp = (int)to_scalar((uint32_t)s.first / (uint32_t)p.page_size);
-        const int32_t id = pages.get(p.page_table, p.max_pages, lp, lane);
-        const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
-        const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
-        s.there = kb != nullptr && vb != nullptr;
-        const int64_t at = (int64_t)(s.first - lp * p.page_size + s.from) * col_bytes + kvh * T::RB;
-        const int bytes = s.there ? (s.to - s.from - 1) * col_bytes + T::RB : 0;
-        const int back = s.from * col_bytes;
-        if constexpr (kQ8) {
-            // nine words from the block's first multiple of 4
-            const int off = u_row * col_bytes + kQ8Bytes * u_blk - 2 * (u_blk & 1) - back;
+    auto load_v = [&](const Src &s, int buf) {
+        const auto r = buffer_of(s.v, s.bytes);
 #pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const auto r = buffer_of(s.there ? ((UN == 2 ? u == 0 : wave < 2) ? kb : vb) + at : nullptr, bytes);
-                const intx4 a = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
-                const intx4 b = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 16, 0));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[u][i] = a[i], raw[u][4 + i] = b[i];
-                raw[u][8] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 32, 0);
-            }
-        } else {
-            const auto kr = buffer_of(s.there ? kb + at : nullptr, bytes);
-            const auto vr = buffer_of(s.there ? vb + at : nullptr, bytes);
-            const uint32_t to = lds_addr(lds[buf][0]) + 1024 * T::NI * wave;
-#pragma unroll
-            for (int i = 0; i < T::NI; ++i) load_to_lds(kr, to + 1024 * i, k_off[i] - back);
-#pragma unroll
-            for (int i = 0; i < T::NI; ++i) load_to_lds(vr, to + T::BYTES + 1024 * i, v_off[i] - back);
-        }
-        return s;
-    };
-    // Q8_0: a block from registers to LDS: K's quants as f16 and their scale
-    // beside them; V's values, under the power of two of the largest scale of
-    // the wave's rows, as two f16
-    auto stage = [&]() {
-        if constexpr (kQ8) {
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const bool is_v = UN == 2 ? u == 1 : wave >= 2;
-                uint32_t w[9];
-#pragma unroll
-                for (int i = 0; i < 9; ++i) w[i] = raw[u][i];
-                const bool odd = u_blk & 1;  // d in the upper half of the first word, quants from the second on
-                float d = (float)__builtin_bit_cast(_Float16, (uint16_t)(odd ? w[0] >> 16 : w[0]));
-                uint32_t qw[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    qw[i] = odd ? w[i + 1] : __builtin_amdgcn_alignbyte(w[i + 1], w[i], 2);
-                if (is_v) {
-                    const bool bad = !(fabsf(d) < INFINITY);
-                    d = bad ? 0.0f : d;
-                    const uint64_t bads = __ballot(bad);
-                    const float big = wave_max(fabsf(d));
-                    const int e = max((int)(__builtin_bit_cast(uint32_t, big) >> 23), 1);
-                    if (lane == 0) {
-                        v_bad[0][wave] = bads;
-                        if constexpr (NB == 4) v_exp[wave] = e;
-                        else v_exp[2 * (wave - 2)] = v_exp[2 * (wave - 2) + 1] = e;
-                    }
-                    const float x = __builtin_amdgcn_ldexpf(d, 127 - e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        half8 h, l;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int q = (int)(int8_t)(qw[2 * i + j / 4] >> 8 * (j % 4));
-                            _Float16 a, b;
-                            split_f16(x * (float)q, a, b);
-                            h[j] = a;
-                            l[j] = b;
-                        }
-                        const int at = u_row * T::ROW + 16 * pv_slot<KVT, HD>(u_row, 4 * u_blk + i);
-                        *reinterpret_cast<half8 *>(&lds[0][1][at]) = h;
-                        *reinterpret_cast<half8 *>(&lds[0][SETS - 1][at]) = l;
-                    }
-                } else {
-                    k_scale[u_blk][u_row] = d;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        half8 h;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) h[j] = (_Float16)(int)(int8_t)(qw[2 * i + j / 4] >> 8 * (j % 4));
-                        *reinterpret_cast<half8 *>(&lds[0][0][u_row * T::ROW + 16 * pk_slot<KVT, HD>(u_row, 4 * u_blk + i)]) = h;
-                    }
-                }
-            }
-        }
+        for (int i = 0; i < T::NI; ++i)
+            load_to_lds(r, my_lds + buf * T::BYTES + 1024 * i, row_off + (i * RPI * col_bytes - s.back) + v_chunk);
     };
 
     // probabilities are 2^(s f - base), base kSplitShift below the row's running
-    // maximum (F32: at it); l sums this lane's
-    constexpr float SHIFT = kF32 ? 0.0f : (float)kSplitShift;
+    // maximum; l sums this lane's
     float base = -INFINITY, l = 0.0f;
-    int unit_exp = 1;  // Q8_0: o is in units of 2^(unit_exp - 127), the largest V scale's so far
     floatx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    floatx16 s[PB];
 
-    Src src = {}, next = {};
-    if (t0 < t1) src = issue(t0, 0);
-    int buf = 0;
-    for (int t = t0; t < t1; ++t, buf ^= BUFS - 1, src = next) {
-        // masked where a row of the workgroup does not see the whole tile
-        const int end = src.first + TP - 1;
-        const bool masked = (src.from > 0) | (src.to < TP) |
-                            (!src.sink & ((end > first) | ((src.first <= last - p.window) & (end >= p.n_sink))));
-        if constexpr (kQ8) {
-            __syncthreads();  // the last tile has been read
-            stage();
-            if (t + 1 < t1) next = issue(t + 1, 0);
-            __syncthreads();
-        } else {
-            wait_loads<0>();
-            // a value that is not finite would reach rows that do not see it, as
-            // 0 times it: the wave looks its quarter of V over
-            if (masked) {
-                bool any = false;
+    // Operand addresses: a step's are these with its chunk XORed in (the slots
+    // are XORs too) and its rows added.
+    const int li = lane & 15, vr = 4 * hh + (li >> 2);
+    const int k_row = n * T::ROW + 16 * pk_slot<HD>(n, hh);
+    const int v_row = vr * T::ROW + 16 * pv_slot<HD>(vr, 2 * (lane >> 4 & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
+    // Operand of step (st, d): positions 16 st + 4 hh .. and 16 st + 8 + 4 hh ..,
+    // the lane's own scores; four values a read, lane i of 16 gets dim i of the
+    // four rows its group names.
+    auto v_at = [&](int v_base, int i) {
+        const uint8_t *const at = &lds[0][0] + (v_base ^ (64 * (i % DB))) + 16 * (i / DB) * T::ROW;
+        const half4 x = tr16_read(at), y = tr16_read(at + 8 * T::ROW);
+        return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+    auto tile = [&](const Src &src, int par) {
+        int k_base = k_row + par * T::BYTES;
+        asm("" : "+v"(k_base));  // keeps the compiler from holding every step's address
 #pragma unroll
-                for (int i = 0; i < T::NI; ++i) {
-                    const int ch = (T::NI * wave + i) * 64 + lane;
-                    intx4 *const at = reinterpret_cast<intx4 *>(&lds[buf][1][16 * ch]);
-                    intx4 x = *at;
-                    uint32_t bits = 0;
+        for (int x = 0; x < PB; ++x)
 #pragma unroll
-                    for (int j = 0; j < (kF32 ? 4 : 8); ++j) {
-                        const uint32_t e = kF32 ? (uint32_t)x[j & 3] >> 23 & 255 : (uint32_t)x[j / 2] >> (j % 2 ? 26 : 10) & 31;
-                        bits |= (e == (kF32 ? 255u : 31u) ? 1u : 0u) << j;
-                    }
-                    if (bits != 0) {
+            for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+        pipelined<KC * PB, 3>(
+            [&](int i) { return *reinterpret_cast<const half8 *>(&lds[0][0] + (k_base ^ (32 * (i / PB))) + i % PB * 32 * T::ROW); },
+            [&](int i, half8 a) {
+                const int c = i / PB, x = i % PB;
+                s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], s[x], 0, 0, 0);
+                s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], s[x], 0, 0, 0);
+            });
+        if (src.masked) {
+            int h4 = 4 * hh;
+            asm("" : "+v"(h4));  // (not 32 row numbers held over the loop)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            if constexpr (kF32) x[j] = bits >> j & 1 ? 0 : x[j];
-                            else x[j] &= (bits >> 2 * j & 1 ? 0 : 0xffff) | (bits >> (2 * j + 1) & 1 ? 0 : (int)0xffff0000);
-                        }
-                        *at = x;
-                        any = true;
-                    }
-                    v_bits[buf][ch] = (uint8_t)bits;
-                }
-                const uint64_t who = __ballot(any);
-                if (lane == 0) v_bad[buf][wave] = who;
-            }
-            __syncthreads();  // this tile is there, and the other buffer has been read
-            if (t + 1 < t1) next = issue(t + 1, buf ^ 1);
+            for (int i = 0; i < 16 * PB; ++i)
+                s[i / 16][i % 16] = sees(p, src, i / 16 * 32 + i / 4 % 4 * 8 + h4 + i % 4, b.tpos) ? s[i / 16][i % 16] : -INFINITY;
         }
-        if (!wave_ok || !src.there) continue;
-        const uint8_t *const kt = lds[kQ8 ? 0 : buf][0], *const vt = lds[kQ8 ? 0 : buf][1];
-        // This lane's first operand addresses; a step's are these with its chunk
-        // XORed in (the slots are XORs too) and its rows added.  The empty asm
-        // keeps the compiler from holding every step's address over the loop.
-        int k_at = n * T::ROW + 16 * pk_slot<KVT, HD>(n, hh), v_at0 = 0;
-        const int li = lane & 15;
-        if constexpr (kF32) {
-            v_at0 = 4 * hh * T::ROW + 16 * pv_slot<KVT, HD>(4 * hh, n / 4) + 4 * (n & 3);
-        } else {
-            const int r = 4 * hh + (li >> 2);
-            v_at0 = r * T::ROW + 16 * pv_slot<KVT, HD>(r, 2 * (lane >> 4 & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
-        }
-        asm("" : "+v"(k_at), "+v"(v_at0));
-
-        floatx16 s[PB];
+        float mx = -INFINITY, x, y;
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-        if constexpr (kF32) {
-            pipelined<2 * KC, 3>([&](int c) { return *reinterpret_cast<const floatx4 *>(kt + (k_at ^ (32 * c))); },
-                                 [&](int c, floatx4 a) {
-#pragma unroll
-                                     for (int i = 0; i < 4; ++i)
-                                         s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], qf[c / 2][c % 2 * 4 + i], s[0], 0, 0, 0);
-                                 });
-        } else if constexpr (!kQ8) {
-            pipelined<KC * PB, 3>(
-                [&](int i) {
-                    return *reinterpret_cast<const half8 *>(kt + (k_at ^ (32 * (i / PB))) + i % PB * 32 * T::ROW);
-                },
-                [&](int i, half8 a) {
-                    const int c = i / PB, b = i % PB;
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], s[b], 0, 0, 0);
-                });
-        } else {
-            // two steps a block, then the block's scales
-            floatx16 x;
-            pipelined<KC * PB, 3>(
-                [&](int i) {
-                    const int b = i / 2 % PB, c = i / (2 * PB) * 2 + i % 2;
-                    return *reinterpret_cast<const half8 *>(kt + (k_at ^ (32 * c)) + b * 32 * T::ROW);
-                },
-                [&](int i, half8 a) {
-                    const int b = i / 2 % PB, nb = i / (2 * PB), c = 2 * nb + i % 2;
-                    if (i % 2 == 0)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], x, 0, 0, 0);
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], x, 0, 0, 0);
-                    if (i % 2 == 0) return;
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        const floatx4 d = *reinterpret_cast<const floatx4 *>(&k_scale[nb][32 * b + 8 * i4 + 4 * hh]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[b][4 * i4 + j] = fmaf(x[4 * i4 + j], d[j], s[b][4 * i4 + j]);
-                    }
-                });
-        }
-
-        if (masked) {
-#pragma unroll
-            for (int i = 0; i < 16 * PB; ++i) {
-                const int r = i / 16 * 32 + i / 4 % 4 * 8 + 4 * hh + i % 4, pos = src.first + r;
-                const bool see = (r >= src.from) & (r < src.to) & (pos <= tpos) & (src.sink | (pos > tpos - p.window) | (pos < p.n_sink));
-                s[i / 16][i % 16] = see ? s[i / 16][i % 16] : -INFINITY;
-            }
-        }
-        float mx = -INFINITY, ma, mb;
-#pragma unroll
-        for (int b = 0; b < PB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-        swap_halves(mx, ma, mb);
-        mx = fmaxf(ma, mb) * f - SHIFT;
+        for (int i = 0; i < 16 * PB; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+        swap_halves(mx, x, y);
+        mx = fmaxf(x, y) * f - (float)kSplitShift;
         if (__ballot(mx > base) != 0) {
             const float nb = fmaxf(mx, base);
             const float a = nb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - nb);
@@ -416,114 +343,361 @@ __global__ __launch_bounds__(256, 2) void window_prefill_kernel(WindowParams p) 
             base = nb;
         }
         const float sub = base == -INFINITY ? 0.0f : base;
+        half8 ph[ST], pl[ST];
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
+        for (int st = 0; st < ST; ++st)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], f, -sub));
-                l += s[b][i];
+            for (int j = 0; j < 8; j += 2) {
+                const int e = 8 * st + j;
+                const float u = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], f, -sub));
+                const float v = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16 + 1], f, -sub));
+                l += u + v;
+                half2v h, r;
+                split2_f16(u, v, h, r);
+                ph[st][j] = h[0], ph[st][j + 1] = h[1];
+                pl[st][j] = r[0], pl[st][j + 1] = r[1];
             }
+        int v_base = v_row + (2 + par) * T::BYTES;
+        asm("" : "+v"(v_base));
+        pipelined<ST * DB, 3>([&](int i) { return v_at(v_base, i); },
+                              [&](int i, half8 a) {
+                                  const int st = i / DB, d = i % DB;
+                                  o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
+                                  o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
+                              });
+        if (src.masked && any_bad(v_bad[par]))
+            spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int e) { return (bool)(v_bits[par][r * T::CPR + pv_slot<HD>(r, e / 8)] >> e % 8 & 1); });
+    };
 
-        // A value that is not finite, in a position that some rows may not see:
-        // the products take it as zero; the rows that see it get what it comes
-        // to, NaN.
-        auto spoil = [&]() {
-            for (int r = src.from; r < src.to; ++r) {
-                const int pos = src.first + r;
-                const bool see = (pos <= tpos) & (src.sink | (pos > tpos - p.window) | (pos < p.n_sink));
+    Src cur = {}, next = {};
+    auto issue = [&](int t, int par) {
+        const Src src = source<TP, T::RB>(p, b, pages, t, lane);
+        load_k(src, par);
+        load_v(src, 2 + par);
+        return src;
+    };
+    if (b.t0 < b.t1) cur = issue(b.t0, 0);
+    int par = 0;
+    for (int t = b.t0; t < b.t1; ++t, par ^= 1, cur = next) {
+        wait_loads<0>();
+        if (cur.masked) look_over<HD>(lds[2 + par], v_bits[par], v_bad[par], wave, lane);
+        __syncthreads();  // this tile is there, and the other buffers have been read
+        if (t + 1 < b.t1) next = issue(t + 1, par ^ 1);
+        if (b.wave_ok && cur.there) tile(cur, par);
+    }
+    store_row<HD>(p, b, hh, o, base, l, 1.0f);
+}
+
+// The F32 and Q8_0 kernel: caches whose values are wider than an f16.  A tile
+// waits in registers while the last one is computed and goes to LDS as f16:
+// - F32: K and V as two f16 each, a row of K and eight rows of V under the
+//   power of two of their largest value;
+// - Q8_0: K's quants, whose blocks' scales multiply the scores of a block; V's
+//   values (a quant times its scale) as two f16, exactly.
+// Three products then stand for one of 32 bits (hi hi, hi lo, lo hi; QK of
+// Q8_0 needs two).  A 32-bit matrix instruction is 16 times slower than an f16
+// one.
+template <int KVT, int HD, int G>
+__global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParams p) {
+    using T = PTile<KVT, HD>;
+    constexpr int TP = T::TP, PB = TP / 32, DB = HD / 32, KC = HD / 16, NB = HD / kQK, ST = TP / 16;
+    constexpr bool kQ8 = KVT == SFA_KV_Q8_0;
+    constexpr int SETS = kQ8 ? 3 : 4;               // K (F32: and its lower halves), V, V's lower halves
+    constexpr int V_SHIFT = kQ8 ? 7 : kSplitShift;  // V's largest scale goes to 2^7, its largest value to 2^14
+    constexpr int FENCE = kQ8 ? 0x7f6 : 0x406;      // Q8_0 has loads and arithmetic of its scales between the products
+    __shared__ __attribute__((aligned(256))) uint8_t lds[SETS][T::BYTES];
+    __shared__ __attribute__((aligned(16))) float k_scale[kQ8 ? NB : 1][TP];
+    __shared__ int v_exp[4];                        // exponent of the largest of V: F32: of each 8 positions, Q8_0: of each 16
+    __shared__ uint64_t v_bad[4];                   // lanes of a wave with values of V that are not finite, held as zeros
+    __shared__ uint16_t v_bits[kQ8 ? 4 : 256];      // F32: a bit for each such value of a thread
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hh = lane >> 5;
+    const Block b = block_of<G, TP>(p, wave, n);
+    PageWindow pages;
+    page_window<TP>(p, b, pages, lane);
+    half8 qh[KC], ql[KC];
+    const float f = p.scale_log2 * split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql);
+
+    // What a thread brings of a tile.  F32: 1/8 of a row of K and of V.  Q8_0: a
+    // block; with HD 128 one of K and one of V, with HD 64 the first two waves
+    // have K's and the others V's.
+    const int col_bytes = p.n_head_kv * T::RB;
+    constexpr int FPT = HD / 8;
+    constexpr int UN = kQ8 ? NB / 2 : 2, WORDS = kQ8 ? 9 : FPT;
+    const int unit = kQ8 && NB == 2 ? threadIdx.x & 127 : threadIdx.x;
+    const int u_row = kQ8 ? unit / NB : unit / 8, u_blk = kQ8 ? unit % NB : unit % 8;
+    // (a block's nine words start at its first multiple of 4)
+    const int u_off = u_row * col_bytes + (kQ8 ? kQ8Bytes * u_blk - 2 * (u_blk & 1) : 4 * FPT * u_blk);
+    uint32_t raw[UN][WORDS];
+    auto issue = [&](int t) {
+        const Src s = source<TP, T::RB>(p, b, pages, t, lane);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    if constexpr (kQ8) {
-                        const int u = r * NB + d;  // its unit, NB / 2 * 128 of them in the waves that hold V
-                        const bool bad = v_bad[0][(NB == 4 ? 0 : 2) + u / 64] >> u % 64 & 1;
+        for (int u = 0; u < UN; ++u) {
+            const auto r = buffer_of((UN == 2 ? u == 0 : wave < 2) ? s.k : s.v, s.bytes);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] = bad && see ? NAN : o[d][i];
-                        continue;
+            for (int i = 0; i + 4 <= WORDS; i += 4) {
+                const intx4 x = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(r, u_off - s.back, 4 * i, 0));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[u][i + j] = x[j];
+            }
+            if constexpr (WORDS % 4 != 0) raw[u][WORDS - 1] = __builtin_amdgcn_raw_buffer_load_b32(r, u_off - s.back, 4 * (WORDS - 1), 0);
+        }
+        return s;
+    };
+    auto stage_q8 = [&]() {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const bool is_v = UN == 2 ? u == 1 : wave >= 2;
+            const uint32_t *const w = raw[u];
+            const bool odd = u_blk & 1;  // d in the upper half of the first word, quants from the second on
+            float d = (float)__builtin_bit_cast(_Float16, (uint16_t)(odd ? w[0] >> 16 : w[0]));
+            uint32_t qw[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qw[i] = odd ? w[i + 1] : __builtin_amdgcn_alignbyte(w[i + 1], w[i], 2);
+            if (is_v) {
+                const bool bad = !(fabsf(d) < INFINITY);
+                d = bad ? 0.0f : d;
+                const uint64_t who = __ballot(bad);
+                const int e = max((int)(__builtin_bit_cast(uint32_t, wave_max(fabsf(d))) >> 23), 1);
+                if (lane == 0) {
+                    v_bad[wave] = who;
+                    if constexpr (NB == 4) v_exp[wave] = e;
+                    else v_exp[2 * (wave - 2)] = v_exp[2 * (wave - 2) + 1] = e;
+                }
+                // a scale of 11 bits times a quant of 8: an f16 and what it leaves, which is an f16 too
+                const _Float16 x = (_Float16)__builtin_amdgcn_ldexpf(d, 127 + V_SHIFT - e);
+                const half2v x2 = {x, x};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const half8 q = quants8(qw[2 * i], qw[2 * i + 1]);
+                    half8 h, r;
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const half2v q2 = {q[j], q[j + 1]}, h2 = q2 * x2, r2 = __builtin_elementwise_fma(q2, x2, -h2);
+                        h[j] = h2[0], h[j + 1] = h2[1];
+                        r[j] = r2[0], r[j + 1] = r2[1];
                     }
+                    const int at = u_row * T::ROW + 16 * pv_slot<HD>(u_row, 4 * u_blk + i);
+                    *reinterpret_cast<half8 *>(&lds[SETS - 2][at]) = h;
+                    *reinterpret_cast<half8 *>(&lds[SETS - 1][at]) = r;
+                }
+            } else {
+                k_scale[u_blk][u_row] = d;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int e = 32 * d + i / 4 * 8 + 4 * hh + i % 4;  // the dim of o[d][i]
-                        constexpr int PC = kF32 ? 4 : 8;                    // values of a chunk
-                        const bool bad = v_bits[buf][r * T::CPR + pv_slot<KVT, HD>(r, e / PC)] >> e % PC & 1;
-                        o[d][i] = (bad & see) ? NAN : o[d][i];
-                    }
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<half8 *>(&lds[0][u_row * T::ROW + 16 * pk_slot<HD>(u_row, 4 * u_blk + i)]) = quants8(qw[2 * i], qw[2 * i + 1]);
+            }
+        }
+    };
+    auto stage_f32 = [&]() {
+        // 1/8 of a row as halves: 2 FPT bytes, chunks of 16 (HD 32: half a chunk)
+        auto put = [&](const float (&x)[FPT], uint8_t *hi, uint8_t *lo, bool v) {
+#pragma unroll
+            for (int i = 0; i < FPT; i += FPT < 8 ? 4 : 8) {
+                half2v h[4], r[4];
+#pragma unroll
+                for (int j = 0; j < (FPT < 8 ? 2 : 4); ++j) split2_f16(x[i + 2 * j], x[i + 2 * j + 1], h[j], r[j]);
+                const int e = FPT * u_blk + i, ch = e / 8, in = e % 8 * 2;
+                const int at = u_row * T::ROW + 16 * (v ? pv_slot<HD>(u_row, ch) : pk_slot<HD>(u_row, ch)) + in;
+                if constexpr (FPT < 8) {
+                    *reinterpret_cast<half4 *>(hi + at) = half4{h[0][0], h[0][1], h[1][0], h[1][1]};
+                    *reinterpret_cast<half4 *>(lo + at) = half4{r[0][0], r[0][1], r[1][0], r[1][1]};
+                } else {
+                    *reinterpret_cast<half8 *>(hi + at) = half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+                    *reinterpret_cast<half8 *>(lo + at) = half8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
                 }
             }
         };
-        if constexpr (kF32) {
-            // rows 8 (i / 4) + 4 hh + i % 4: the slots of all are those of row 4 hh
-            pipelined<16 * DB, 4>(
-                [&](int i) { return *reinterpret_cast<const float *>(vt + (v_at0 ^ (128 * (i % DB))) + (i / DB / 4 * 8 + i / DB % 4) * T::ROW); },
-                [&](int i, float a) { o[i % DB] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][i / DB], o[i % DB], 0, 0, 0); });
-        } else {
-            constexpr int ST = TP / 16;  // 16-position steps
-            float w16[ST];
-            if constexpr (kQ8) {
-                int e = unit_exp;
+        float x[FPT], amax = 0.0f, down, up;
 #pragma unroll
-                for (int st = 0; st < ST; ++st) e = max(e, __builtin_amdgcn_readfirstlane(v_exp[st]));
-                if (e > unit_exp) {
-                    const float a = __builtin_amdgcn_ldexpf(1.0f, unit_exp - e);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) o[d] *= a;
-                    unit_exp = e;
-                }
-#pragma unroll
-                for (int st = 0; st < ST; ++st)
-                    w16[st] = __builtin_amdgcn_ldexpf(1.0f, __builtin_amdgcn_readfirstlane(v_exp[st]) - unit_exp);
-            }
-            half8 ph[ST], pl[ST];
-#pragma unroll
-            for (int st = 0; st < ST; ++st)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    _Float16 a, b;
-                    split_f16(kQ8 ? s[st / 2][st % 2 * 8 + j] * w16[st] : s[st / 2][st % 2 * 8 + j], a, b);
-                    ph[st][j] = a;
-                    pl[st][j] = b;
-                }
-            // operand of step st: positions 16 st + 4 hh .. and 16 st + 8 + 4 hh .., the lane's own
-            // scores; four values a read, lane i of 16 gets dim i of the four rows its group names
-            auto v_at = [&](const uint8_t *tile, int st, int d) {
-                const uint8_t *const at = tile + (v_at0 ^ (64 * d)) + 16 * st * T::ROW;
-                const half4 x = tr16_read(at), y = tr16_read(at + 8 * T::ROW);
-                return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            };
-            pipelined<ST * DB, 3>([&](int i) { return v_at(vt, i / DB, i % DB); },
-                                  [&](int i, half8 a) {
-                                      const int st = i / DB, d = i % DB;
-                                      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[st], o[d], 0, 0, 0);
-                                      o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
-                                      if constexpr (kQ8) {
-                                          const half8 b = v_at(lds[0][SETS - 1], st, d);
-                                          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[st], o[d], 0, 0, 0);
-                                      }
-                                  });
+        for (int i = 0; i < FPT; ++i) {
+            x[i] = __builtin_bit_cast(float, raw[0][i]);
+            amax = fmaxf(amax, fabsf(x[i]));
         }
-        if (kQ8 || masked) {
-            const uint64_t *const vb = v_bad[buf];
-            const uint64_t any = kQ8 && NB == 2 ? vb[2] | vb[3] : vb[0] | vb[1] | vb[2] | vb[3];
-            if (__ballot(any != 0) != 0) spoil();
+        amax = fmaxf(amax, dpp_row<0xB1>(amax));  // the row's eight lanes
+        amax = fmaxf(amax, dpp_row<0x4E>(amax));
+        amax = fmaxf(amax, dpp_row<0x141>(amax));
+        row_exponent(amax, down, up);
+        if (u_blk == 0) k_scale[0][u_row] = up;
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) x[i] *= down;
+        put(x, lds[0], lds[1], false);
+        uint32_t bits = 0;
+        amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) {
+            x[i] = __builtin_bit_cast(float, raw[UN - 1][i]);
+            const bool bad = !(fabsf(x[i]) < INFINITY);
+            bits |= (bad ? 1u : 0u) << i;
+            x[i] = bad ? 0.0f : x[i];
+            amax = fmaxf(amax, fabsf(x[i]));
         }
-    }
-    if (!row_ok) return;
-    float la, lb;
-    swap_halves(l, la, lb);
-    l = la + lb;
-    float w = p.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-    if constexpr (kQ8) w = w == 0.0f ? 0.0f : w * __builtin_amdgcn_ldexpf(1.0f, unit_exp - 127);
-    const int64_t out_row = (int64_t)tok * p.n_head + head;
-    float *const dst = p.n_split > 1 ? p.rec_o + (out_row * p.n_split + split) * HD : p.out + out_row * HD;
+        const uint64_t who = __ballot(bits != 0);
+        const int e = max((int)(__builtin_bit_cast(uint32_t, wave_max(amax)) >> 23), 1);
+        if (lane == 0) v_bad[wave] = who, v_exp[wave] = e;
+        if (who != 0) v_bits[threadIdx.x] = (uint16_t)bits;
+#pragma unroll
+        for (int i = 0; i < FPT; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], 127 + V_SHIFT - e);
+        put(x, lds[SETS - 2], lds[SETS - 1], true);
+    };
+
+    // probabilities are 2^(s f - base), base kSplitShift below the row's running
+    // maximum; l sums this lane's; o is in units of 2^(unit_exp - 127 - V_SHIFT),
+    // unit_exp the exponent of the largest of V so far
+    float base = -INFINITY, l = 0.0f;
+    int unit_exp = 1;
+    floatx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-            floatx4 x;
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    struct Two {
+        half8 hi, lo;
+    };
+
+    Src src = {}, next = {};
+    if (b.t0 < b.t1) src = issue(b.t0);
+    for (int t = b.t0; t < b.t1; ++t, src = next) {
+        __syncthreads();  // the last tile has been read
+        if constexpr (kQ8) stage_q8();
+        else stage_f32();
+        if (t + 1 < b.t1) next = issue(t + 1);
+        __syncthreads();
+        if (!b.wave_ok || !src.there) continue;
+        // This lane's first operand addresses; a step's are these with its chunk
+        // XORed in (the slots are XORs too) and its rows added.  The empty asm
+        // keeps the compiler from holding every step's address over the loop.
+        const int li = lane & 15, vr = 4 * hh + (li >> 2);
+        int k_at = n * T::ROW + 16 * pk_slot<HD>(n, hh);
+        int v_at = vr * T::ROW + 16 * pv_slot<HD>(vr, 2 * (lane >> 4 & 1) + ((li & 3) >> 1)) + 8 * (li & 1);
+        asm("" : "+v"(k_at), "+v"(v_at));
+
+        floatx16 s[PB];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = o[d][4 * i4 + i] * w;
-            *reinterpret_cast<floatx4 *>(dst + 32 * d + 8 * i4 + 4 * hh) = x;
+        for (int x = 0; x < PB; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+        if constexpr (!kQ8) {
+            pipelined<KC, 2, FENCE>(
+                [&](int c) {
+                    const uint8_t *const at = &lds[0][0] + (k_at ^ (32 * c));
+                    return Two{*reinterpret_cast<const half8 *>(at), *reinterpret_cast<const half8 *>(at + T::BYTES)};
+                },
+                [&](int c, Two a) {
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hi, qh[c], s[0], 0, 0, 0);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hi, ql[c], s[0], 0, 0, 0);
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.lo, qh[c], s[0], 0, 0, 0);
+                });
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const floatx4 d = *reinterpret_cast<const floatx4 *>(&k_scale[0][8 * i4 + 4 * hh]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[0][4 * i4 + j] *= d[j];
+            }
+        } else {
+            // two steps a block, then the block's scales
+            floatx16 x;
+            pipelined<KC * PB, 3, FENCE>(
+                [&](int i) {
+                    const int blk = i / 2 % PB, c = i / (2 * PB) * 2 + i % 2;
+                    return *reinterpret_cast<const half8 *>(&lds[0][0] + (k_at ^ (32 * c)) + blk * 32 * T::ROW);
+                },
+                [&](int i, half8 a) {
+                    const int blk = i / 2 % PB, nb = i / (2 * PB), c = 2 * nb + i % 2;
+                    if (i % 2 == 0)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], x, 0, 0, 0);
+                    if (i % 2 == 0) return;
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        const floatx4 d = *reinterpret_cast<const floatx4 *>(&k_scale[nb][32 * blk + 8 * i4 + 4 * hh]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[blk][4 * i4 + j] = fmaf(x[4 * i4 + j], d[j], s[blk][4 * i4 + j]);
+                    }
+                });
         }
-    if (p.n_split > 1 && hh == 0) p.rec_ml[out_row * p.n_split + split] = make_float2(base, l);
+        if (src.masked) {
+            int h4 = 4 * hh;
+            asm("" : "+v"(h4));  // (not 32 row numbers held over the loop)
+#pragma unroll
+            for (int i = 0; i < 16 * PB; ++i)
+                s[i / 16][i % 16] = sees(p, src, i / 16 * 32 + i / 4 % 4 * 8 + h4 + i % 4, b.tpos) ? s[i / 16][i % 16] : -INFINITY;
+        }
+        float mx = -INFINITY, ma, mb;
+#pragma unroll
+        for (int x = 0; x < PB; ++x)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+        swap_halves(mx, ma, mb);
+        mx = fmaxf(ma, mb) * f - (float)kSplitShift;
+        int exps[4], e = unit_exp;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            exps[i] = __builtin_amdgcn_readfirstlane(v_exp[i]);
+            e = max(e, exps[i]);
+        }
+        if (__ballot(mx > base) != 0 || e > unit_exp) {
+            const float nb = fmaxf(mx, base);
+            const float a = nb == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(base - nb);
+            const float a_o = __builtin_amdgcn_ldexpf(a, unit_exp - e);
+            l *= a;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= a_o;
+            base = nb;
+            unit_exp = e;
+        }
+        const float sub = base == -INFINITY ? 0.0f : base;
+        half8 ph[ST], pl[ST];
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const int i = 8 * st + j;
+                const float u = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16], f, -sub));
+                const float v = __builtin_amdgcn_exp2f(fmaf(s[i / 16][i % 16 + 1], f, -sub));
+                l += u + v;
+                // to the units of o, by a power of two: F32: values j < 4 are of positions 16 st .. + 7
+                const int w = exps[kQ8 ? st : 2 * st + j / 4] - unit_exp;
+                half2v h, r;
+                split2_f16(__builtin_amdgcn_ldexpf(u, w), __builtin_amdgcn_ldexpf(v, w), h, r);
+                ph[st][j] = h[0], ph[st][j + 1] = h[1];
+                pl[st][j] = r[0], pl[st][j + 1] = r[1];
+            }
+        // operand of step st: positions 16 st + 4 hh .. and 16 st + 8 + 4 hh .., the lane's own
+        // scores; four values a read, lane i of 16 gets dim i of the four rows its group names
+        auto v_read = [&](int set, int st, int d) {
+            const uint8_t *const at = &lds[set][0] + (v_at ^ (64 * d)) + 16 * st * T::ROW;
+            const half4 x = tr16_read(at), y = tr16_read(at + 8 * T::ROW);
+            return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        };
+        pipelined<ST * DB, 2, FENCE>([&](int i) { return Two{v_read(SETS - 2, i / DB, i % DB), v_read(SETS - 1, i / DB, i % DB)}; },
+                                     [&](int i, Two a) {
+                                         const int st = i / DB, d = i % DB;
+                                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hi, ph[st], o[d], 0, 0, 0);
+                                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hi, pl[st], o[d], 0, 0, 0);
+                                         o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.lo, ph[st], o[d], 0, 0, 0);
+                                     });
+        if constexpr (kQ8) {
+            // units of V: NB / 2 * 128 of them in the waves that hold V
+            constexpr int W0 = NB == 4 ? 0 : 2;
+            if (__ballot((v_bad[W0] | v_bad[W0 + 1] | v_bad[2] | v_bad[3]) != 0) != 0)
+                spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int d) {
+                    const int u = r * NB + d / kQK;
+                    return (bool)(v_bad[W0 + u / 64] >> u % 64 & 1);
+                });
+        } else {
+            if (any_bad(v_bad))
+                spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int d) {
+                    const int th = r * 8 + d / FPT;
+                    return (bool)((v_bad[th / 64] >> th % 64 & 1) & (v_bits[th] >> d % FPT & 1));
+                });
+        }
+    }
+    store_row<HD>(p, b, hh, o, base, l, __builtin_amdgcn_ldexpf(1.0f, unit_exp - 127 - V_SHIFT));
 }
 
 // Workgroups that share a row block's tiles: as many as fill the chip's CUs
@@ -540,11 +714,20 @@ int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int3
 template <int KVT, int HD>
 static void launch_g(const WindowParams &p, dim3 grid, hipStream_t s) {
     const dim3 block(256);
+    if constexpr (KVT == SFA_KV_F16) {
+        switch (p.n_head / p.n_head_kv) {
+        case 1: hipLaunchKernelGGL((window_prefill_f16_kernel<HD, 1>), grid, block, 0, s, p); break;
+        case 2: hipLaunchKernelGGL((window_prefill_f16_kernel<HD, 2>), grid, block, 0, s, p); break;
+        case 4: hipLaunchKernelGGL((window_prefill_f16_kernel<HD, 4>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((window_prefill_f16_kernel<HD, 8>), grid, block, 0, s, p); break;
+        }
+        return;
+    } else
     switch (p.n_head / p.n_head_kv) {
-    case 1: hipLaunchKernelGGL((window_prefill_kernel<KVT, HD, 1>), grid, block, 0, s, p); break;
-    case 2: hipLaunchKernelGGL((window_prefill_kernel<KVT, HD, 2>), grid, block, 0, s, p); break;
-    case 4: hipLaunchKernelGGL((window_prefill_kernel<KVT, HD, 4>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((window_prefill_kernel<KVT, HD, 8>), grid, block, 0, s, p); break;
+    case 1: hipLaunchKernelGGL((window_prefill_wide_kernel<KVT, HD, 1>), grid, block, 0, s, p); break;
+    case 2: hipLaunchKernelGGL((window_prefill_wide_kernel<KVT, HD, 2>), grid, block, 0, s, p); break;
+    case 4: hipLaunchKernelGGL((window_prefill_wide_kernel<KVT, HD, 4>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((window_prefill_wide_kernel<KVT, HD, 8>), grid, block, 0, s, p); break;
     }
 }
 
