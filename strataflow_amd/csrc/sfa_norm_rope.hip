@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(NormRopeParams p)
     const bool rot = 8 * l < p.n_rot;
     const int c0 = rot && p.neox ? 4 * l : 8 * l;
     const int c1 = rot && p.neox ? half + 4 * l : 8 * l + 4;
-    for (int r = slot; r < n_rows; r += RPB) {
+    for (int r = slot + blockIdx.y * RPB; r < n_rows; r += RPB * gridDim.y) {
         const int what = r < n_q ? 0 : r < n_q + p.a.n_head_kv ? 1 : 2;  // Q, K or V
         const int h = what == 0 ? r : (r - n_q) % p.a.n_head_kv;
         const float *src = what == 0   ? p.q + tok * p.q_stride
@@ -195,7 +195,10 @@ static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 template <int KVT>
 static int launch_hd(const NormRopeParams &p, hipStream_t s) {
-    const dim3 grid((unsigned)p.a.n_tok), block(256);
+    // few tokens: a workgroup for every 256 lanes' heads, each with its own table
+    // of angles, instead of a loop over them
+    const int rows = (p.q != nullptr ? p.n_head : 0) + 2 * p.a.n_head_kv, pass = 2048 / p.a.head_dim;
+    const dim3 grid((unsigned)p.a.n_tok, p.a.n_tok < 128 ? (unsigned)((rows + pass - 1) / pass) : 1u), block(256);
     if (p.a.head_dim == 128) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 128>), grid, block, 0, s, p);
     else if (p.a.head_dim == 64) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 64>), grid, block, 0, s, p);
     else if constexpr (KVT != SFA_KV_Q8_0) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 32>), grid, block, 0, s, p);

@@ -78,6 +78,7 @@ SFA_API int sfa_attn_decode_window(const sfa_kv_desc *kv, const float *q, float 
         if (ws_bytes < sfa_decode_window_workspace_bytes(kv, B, max_seq_len, window, n_sink))
             return SFA_ERR_INVALID_ARGUMENT;
         p.seq_len = seq_len;
+        p.n_tok = B;
         sfa::set_records(&p, workspace, (int64_t)B * kv->n_head,
                          sfa::window_decode_splits(kv, B, max_seq_len, window, n_sink), kv->head_dim);
         return sfa::window_decode_launch(p, kv, B, static_cast<hipStream_t>(stream));

@@ -29,7 +29,7 @@ struct Tile {
     static constexpr int CPR = (RB + 15) / 16;               // 16-byte chunks of a row (Q8_0 rows end inside one)
     static constexpr int ROW = CPR * 16;                     // row in LDS
     static constexpr int NI = (TP * CPR + kWave - 1) / kWave;  // load instructions
-    static constexpr int BYTES = NI * 1024;
+    static constexpr int BYTES = TP * CPR * 16;
     static constexpr int RP = 256 / ROW > 0 ? 256 / ROW : 1;  // rows under all LDS banks (a power of two but for Q8_0)
 };
 
@@ -51,7 +51,7 @@ __device__ inline int v_slot(int r, int j) {
 }
 
 template <int KVT, int HD, int G>
-__global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowParams p) {
+__global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 2) void window_decode_kernel(WindowParams p) {
     using T = Tile<KVT, HD>;
     constexpr int TP = T::TP, MT = TP / 16;  // 16-position blocks of a tile
     constexpr int KS = HD / 32, DB = HD / 16;
@@ -65,9 +65,15 @@ __global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowPar
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, qd = lane >> 4;
-    const int kvh = blockIdx.x % p.n_head_kv;
-    const int rest = blockIdx.x / p.n_head_kv;
-    const int split = rest % p.n_split, b = rest / p.n_split;
+    // Workgroups go round the eight XCDs.  The rows of neighbouring kv heads share
+    // cache lines in a Q8_0 cache: there the heads of one split are eight apart,
+    // in one L2 (8 sequences, window 8192: the step 59 -> 51 us).  Whole lines are
+    // faster from all over the chip (F16, 64 sequences: 190 us against 200).
+    constexpr bool kShared = KVT == SFA_KV_Q8_0;
+    const int kvh = (kShared ? blockIdx.x / 8 : blockIdx.x) % p.n_head_kv;
+    const int part = kShared ? blockIdx.x / (8 * p.n_head_kv) * 8 + blockIdx.x % 8 : blockIdx.x / p.n_head_kv;
+    const int split = part % p.n_split, b = part / p.n_split;
+    if (b >= p.n_tok) return;  // (the parts of a Q8_0 cache are rounded up to eight)
     const int32_t *table = p.page_table + (int64_t)b * p.max_pages;
     const int len = p.seq_len[b];
 
@@ -106,9 +112,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowPar
 #pragma unroll
     for (int i = 0; i < T::NI; ++i) {
         const int ch = 64 * i + lane, r = ch / T::CPR, j = ch % T::CPR;
-        const bool in = ch < TP * T::CPR;  // the rest of the last instruction loads nothing
-        k_off[i] = in ? r * col_bytes + 16 * k_slot<KVT, HD>(r, j) : -(1 << 30);
-        v_off[i] = in ? r * col_bytes + 16 * v_slot<KVT, HD>(r, j) : -(1 << 30);
+        k_off[i] = r * col_bytes + 16 * k_slot<KVT, HD>(r, j);
+        v_off[i] = r * col_bytes + 16 * v_slot<KVT, HD>(r, j);
     }
     uint8_t *const mine = lds + wave * WAVE;
     const uint32_t mine_at = lds_addr(mine);
@@ -131,10 +136,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowPar
         const auto vr = buffer_of(there ? vb + row : nullptr, bytes);
         const int up = from * col_bytes;
         const uint32_t at = mine_at + buf * STAGE;
+        // (the last instruction of Q8_0 by the lanes that have a chunk left)
+        constexpr int LAST = TP * T::CPR - 64 * (T::NI - 1);
 #pragma unroll
-        for (int i = 0; i < T::NI; ++i) load_to_lds(kr, at + 1024 * i, k_off[i] - up);
+        for (int i = 0; i < T::NI; ++i)
+            if (i < T::NI - 1 || LAST == 64 || lane < LAST) load_to_lds(kr, at + 1024 * i, k_off[i] - up);
 #pragma unroll
-        for (int i = 0; i < T::NI; ++i) load_to_lds(vr, at + T::BYTES + 1024 * i, v_off[i] - up);
+        for (int i = 0; i < T::NI; ++i)
+            if (i < T::NI - 1 || LAST == 64 || lane < LAST) load_to_lds(vr, at + T::BYTES + 1024 * i, v_off[i] - up);
         r0[buf] = from;
         r1[buf] = there ? to : 0;
     };
@@ -403,67 +412,97 @@ __global__ __launch_bounds__(64 * kWaves, 1) void window_decode_kernel(WindowPar
     }
 }
 
-// Joins a row's split records: a thread has four dims of every NG-th split.
-template <int HD>
-__global__ __launch_bounds__(256) void window_merge_kernel(WindowParams p) {
+// Joins a row's split records: a thread has four dims of every GR-th split,
+// GR groups of HD / 4 threads a row.
+template <int HD, int GR>
+__global__ __launch_bounds__(256) void window_merge_kernel(WindowParams p, int64_t rows) {
     constexpr int LN = HD / 4, NG = 256 / LN;
     __shared__ float jm[NG], jl[NG];
     __shared__ floatx4 jo[NG][LN];
-    const int64_t row = blockIdx.x;
     const int grp = threadIdx.x / LN, e = threadIdx.x % LN;
+    const int64_t row = (int64_t)blockIdx.x * (NG / GR) + grp / GR;
+    const bool ok = row < rows;
     const float2 *const ml = p.rec_ml + row * p.n_split;
-    const float *const rec = p.rec_o + row * p.n_split * HD;
+    const float *const rec = p.rec_o + row * p.n_split * HD + 4 * e;
     float m = -INFINITY, l = 0.0f;
     floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s = grp; s < p.n_split; s += NG) {
-        const float2 r = ml[s];
-        const floatx4 x = *reinterpret_cast<const floatx4 *>(rec + (int64_t)s * HD + 4 * e);
-        const float mn = fmaxf(m, r.x), mb = mn == -INFINITY ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - mb), w = __builtin_amdgcn_exp2f(r.x - mb);
-        l = fmaf(r.y, w, l * a);
+    // four splits' loads at a time (a split past the last: the last, of no weight)
+    for (int s = grp % GR; ok && s < p.n_split; s += 4 * GR) {
+        float2 r[4];
+        floatx4 x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], w, o[i] * a);
+        for (int i = 0; i < 4; ++i) {
+            const int at = min(s + i * GR, p.n_split - 1);
+            r[i] = ml[at];
+            x[i] = *reinterpret_cast<const floatx4 *>(rec + (int64_t)at * HD);
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mn = fmaxf(mn, r[i].x);
+        const float mb = mn == -INFINITY ? 0.0f : mn, a = __builtin_amdgcn_exp2f(m - mb);
+        l *= a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] *= a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s + i * GR >= p.n_split) continue;
+            const float w = __builtin_amdgcn_exp2f(r[i].x - mb);
+            l = fmaf(r[i].y, w, l);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(x[i][j], w, o[j]);
+        }
         m = mn;
     }
-    if (e == 0) jm[grp] = m, jl[grp] = l;
-    jo[grp][e] = o;
-    __syncthreads();
-    if (grp != 0) return;
-    float mm = -INFINITY;
+    if constexpr (GR > 1) {
+        if (e == 0) jm[grp] = m, jl[grp] = l;
+        jo[grp][e] = o;
+        __syncthreads();
+        if (grp % GR != 0) return;
+        float mm = -INFINITY;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) mm = fmaxf(mm, jm[g]);
-    if (mm == -INFINITY) mm = 0.0f;
-    float L = 0.0f;
-    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int g = 0; g < GR; ++g) mm = fmaxf(mm, jm[grp + g]);
+        if (mm == -INFINITY) mm = 0.0f;
+        l = 0.0f;
+        o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const float w = __builtin_amdgcn_exp2f(jm[g] - mm);
-        L = fmaf(jl[g], w, L);
+        for (int g = 0; g < GR; ++g) {
+            const float w = __builtin_amdgcn_exp2f(jm[grp + g] - mm);
+            l = fmaf(jl[grp + g], w, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(jo[g][e][i], w, acc[i]);
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(jo[grp + g][e][j], w, o[j]);
+        }
     }
+    if (!ok) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = L == 0.0f ? 0.0f : acc[i] / L;
-    *reinterpret_cast<floatx4 *>(p.out + row * HD + 4 * e) = acc;
+    for (int j = 0; j < 4; ++j) o[j] = l == 0.0f ? 0.0f : o[j] / l;
+    *reinterpret_cast<floatx4 *>(p.out + row * HD + 4 * e) = o;
+}
+
+template <int HD>
+static void launch_merge(const WindowParams &p, int64_t rows, hipStream_t s) {
+    constexpr int NG = 256 / (HD / 4);
+    // few splits are read by one group of threads in one round of loads
+    if (p.n_split <= 4)
+        hipLaunchKernelGGL((window_merge_kernel<HD, 1>), dim3((unsigned)((rows + NG - 1) / NG)), dim3(256), 0, s, p, rows);
+    else
+        hipLaunchKernelGGL((window_merge_kernel<HD, 8>), dim3((unsigned)((rows + NG / 8 - 1) / (NG / 8))), dim3(256), 0, s, p, rows);
 }
 
 int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipStream_t s) {
-    const dim3 grid((unsigned)rows), block(256);
-    if (head_dim == 128) hipLaunchKernelGGL(window_merge_kernel<128>, grid, block, 0, s, p);
-    else if (head_dim == 64) hipLaunchKernelGGL(window_merge_kernel<64>, grid, block, 0, s, p);
-    else hipLaunchKernelGGL(window_merge_kernel<32>, grid, block, 0, s, p);
+    if (head_dim == 128) launch_merge<128>(p, rows, s);
+    else if (head_dim == 64) launch_merge<64>(p, rows, s);
+    else launch_merge<32>(p, rows, s);
     return hipGetLastError() == hipSuccess ? SFA_OK : SFA_ERR_RUNTIME;
 }
 
 // Workgroups of one sequence and kv head: as many as fill the chip once (one
-// workgroup a CU where a row's two buffers take over half its LDS, else two),
-// at most one per four tiles of the longest span.
+// workgroup a CU where its buffers take over half the LDS, else two), at most
+// one per four tiles of the longest span.
 int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink) {
     const int tp = kv->kv_type == SFA_KV_F32 ? 16 : 32;
     const int64_t seen = (int64_t)window + n_sink < max_seq_len ? (int64_t)window + n_sink : max_seq_len;
     const int64_t tiles = (seen + tp - 1) / tp + 2;
-    const int64_t room = kv->head_dim == 128 ? 256 : 512;
+    const int64_t room = kv->head_dim == 128 && kv->kv_type != SFA_KV_Q8_0 ? 256 : 512;
     int64_t n = room / ((int64_t)B * kv->n_head_kv);
     if (n > (tiles + kWaves - 1) / kWaves) n = (tiles + kWaves - 1) / kWaves;
     return n < 1 ? 1 : (int)n;
@@ -490,7 +529,8 @@ static int launch_hd(const WindowParams &p, int head_dim, unsigned grid, hipStre
 }
 
 int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s) {
-    const int64_t grid = (int64_t)B * kv->n_head_kv * p.n_split, rows = (int64_t)B * kv->n_head;
+    const int64_t parts = (int64_t)B * p.n_split;
+    const int64_t grid = (kv->kv_type == SFA_KV_Q8_0 ? (parts + 7) / 8 * 8 : parts) * kv->n_head_kv, rows = (int64_t)B * kv->n_head;
     if (grid > INT32_MAX || rows > INT32_MAX) return SFA_ERR_UNSUPPORTED;
     int rc;
     switch (kv->kv_type) {

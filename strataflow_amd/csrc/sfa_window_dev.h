@@ -22,7 +22,8 @@ struct WindowParams {
     int n_head, n_head_kv, row_bytes;
     const int32_t *page_table;
     const int32_t *seq_len;  // decode; null for a chunk
-    int q_pos0, n_tok;       // chunk
+    int q_pos0;              // chunk
+    int n_tok;               // of the chunk; decode: sequences
     int window, n_sink;
     float scale_log2;        // scale * log2(e): probabilities are powers of two
     int n_split;

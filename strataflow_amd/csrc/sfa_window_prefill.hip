@@ -700,15 +700,32 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
     store_row<HD>(p, b, hh, o, base, l, __builtin_amdgcn_ldexpf(1.0f, unit_exp - 127 - V_SHIFT));
 }
 
-// Workgroups that share a row block's tiles: as many as fill the chip's CUs
-// twice, at most one per two tiles of the block's span.
+// Workgroups that share a row block's tiles: the number with the least estimated
+// time.  A tile takes `tile` us where a CU has one workgroup, `pair` times that
+// where two share it (and in proportion beyond); every split writes and reads
+// its rows' records, at 3.5 TB/s.  Measured (us; 32 / 8 heads of 128): F16 93
+// tokens on 20100, window 4096: 164 / 54 / 37 / 39 with 1 / 4 / 10 / 21; Q8_0
+// 777 on 6000, window 1024: 98 / 83 / 94 with 1 / 2 / 3; F32 (16 / 4 heads) 1500
+// tokens, window 512: 64 / 59 / 67 with 1 / 2 / 4.
 int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int32_t window, int32_t n_sink) {
-    const int tp = kv->kv_type == SFA_KV_F32 ? 32 : 64, g = kv->n_head / kv->n_head_kv;
-    const int64_t blocks = ((int64_t)T * g + kRows - 1) / kRows, span = (int64_t)window + kRows / g + n_sink;
-    const int64_t end = (int64_t)q_pos0 + T, tiles = ((span < end ? span : end) + tp - 1) / tp;
-    int64_t n = 512 / (blocks * kv->n_head_kv);
-    if (n > tiles / 2) n = tiles / 2;
-    return n < 1 ? 1 : (int)n;
+    const bool f32 = kv->kv_type == SFA_KV_F32, f16 = kv->kv_type == SFA_KV_F16;
+    const int tp = f32 ? 32 : 64, g = kv->n_head / kv->n_head_kv;
+    const double tile = (f16 ? 2.5 : f32 ? 3.7 : 5.1) * kv->head_dim / 128, pair = f16 ? 1.6 : 1.4;
+    const int64_t blocks = ((int64_t)T * g + kRows - 1) / kRows * kv->n_head_kv;
+    const int64_t span = (int64_t)window + kRows / g + n_sink, end = (int64_t)q_pos0 + T;
+    const int64_t tiles = ((span < end ? span : end) + tp - 1) / tp;
+    const double record = 2.0 * T * kv->n_head * kv->head_dim * 4 / 3.5e6;
+    int best = 1;
+    double least = 0.0;
+    for (int n = 1; n <= 64 && n <= tiles && (n == 1 || blocks * n <= 1024); ++n) {
+        const int64_t cu = (blocks * n + 255) / 256;
+        const double us = (double)((tiles + n - 1) / n) * tile * (cu == 1 ? 1.0 : pair * cu / 2) + (n > 1 ? 3.0 + n * record : 0.0);
+        if (n == 1 || us < least) {
+            least = us;
+            best = n;
+        }
+    }
+    return best;
 }
 
 template <int KVT, int HD>
