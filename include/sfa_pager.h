@@ -28,6 +28,7 @@
 #define SFA_PAGER_H
 
 #include "sfa.h"
+#include "sfa_window.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -67,6 +68,16 @@ typedef struct sfa_pager_stats {
 /* Allocates the device pool (all layers, K and V), the host-pinned cold pool,
  * the device page tables and the decode workspace.  Synchronises the device. */
 SFA_API int sfa_pager_create(const sfa_pager_config *cfg, sfa_pager **out);
+/* sfa_pager_create for a windowed model (sfa_window.h): every token attends
+ * the `window` positions up to its own and the first n_sink of its sequence.
+ * cfg->attend must be SFA_ATTEND_WINDOW, cfg->window > 0 and n_sink >= 0.  Pages
+ * with one of the first n_sink positions are never released, other pages at the
+ * first step none of whose tokens sees them (so a chunk's first token still
+ * has its whole window).  cfg->n_pages 0 = n_seq * (pages of the window and a
+ * chunk beside the sinks'); cfg->n_cold_pages is not used.  A sequence may take
+ * up to page_size tokens in a step.  sfa_pager_attend runs
+ * sfa_attn_decode_window and sfa_attn_prefill_window. */
+SFA_API int sfa_pager_create_sinks(const sfa_pager_config *cfg, int32_t n_sink, sfa_pager **out);
 SFA_API void sfa_pager_destroy(sfa_pager *pager);
 
 /* Starts a step: sequence b gets the next n_tok[b] positions (0 <= n_tok[b] <=
@@ -96,6 +107,15 @@ SFA_API int sfa_pager_append(sfa_pager *pager, int32_t layer, const float *k, co
 SFA_API int sfa_pager_rope_append(sfa_pager *pager, int32_t layer, float *q, const float *k,
                                   const float *v, float freq_base, void *stream);
 
+/* sfa_pager_append with the head norms and the rotation of Q and K on the way
+ * (sfa_norm_rope_kv_append, whose arguments these are; rope_pos
+ * [n_axis][n_tokens], or NULL for the tokens' positions). */
+SFA_API int sfa_pager_norm_rope_append(sfa_pager *pager, int32_t layer, const sfa_rope_desc *rope,
+                                       const float *q, int64_t q_stride, float *q_out, const float *k,
+                                       int64_t k_stride, const float *v, int64_t v_stride,
+                                       const float *q_norm, const float *k_norm, float eps,
+                                       const int32_t *rope_pos, void *stream);
+
 /* Attention of the step's tokens over one layer: q [n_tokens][n_head][head_dim]
  * f32 device, out [n_tokens][n_head * head_dim] f32 device.  A step with one
  * token per sequence runs sfa_attn_decode over the batch (split plan sized for
@@ -103,7 +123,8 @@ SFA_API int sfa_pager_rope_append(sfa_pager *pager, int32_t layer, float *q, con
  * sfa_attn_prefill per sequence with tokens (its page-size and Q8_0 head_dim
  * limits are checked by sfa_pager_create already).  Under
  * SFA_ATTEND_WINDOW a sequence may take at most one token in such a step (each
- * token of a chunk would need its own window start): SFA_ERR_UNSUPPORTED. */
+ * token of a chunk would need its own window start): SFA_ERR_UNSUPPORTED, but
+ * for pagers of sfa_pager_create_sinks. */
 SFA_API int sfa_pager_attend(sfa_pager *pager, int32_t layer, const float *q, float *out,
                              void *stream);
 

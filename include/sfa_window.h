@@ -107,6 +107,11 @@ SFA_API int sfa_attn_decode_window(const sfa_kv_desc *kv, const float *q, float 
 SFA_API size_t sfa_prefill_window_workspace_bytes(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T,
                                                   int32_t window, int32_t n_sink);
 
+/* Workspace bytes that every sfa_attn_prefill_window of at most max_T tokens
+ * over this cache fits in, whatever its position, window and sinks; 0 where none
+ * needs any, and for an invalid shape. */
+SFA_API size_t sfa_prefill_window_workspace_bound(const sfa_kv_desc *kv, int32_t max_T);
+
 /* Chunk attention of ONE sequence: T query tokens at positions q_pos0 ..
  * q_pos0 + T - 1, whose K/V are appended; the token at position t attends the
  * positions p <= t with p < n_sink or p > t - window.  q, out, page_table,

@@ -63,6 +63,7 @@ WINDOW_EXPORTS = (
     "sfa_decode_window_workspace_bytes",
     "sfa_attn_decode_window",
     "sfa_prefill_window_workspace_bytes",
+    "sfa_prefill_window_workspace_bound",
     "sfa_attn_prefill_window",
 )
 
@@ -188,6 +189,8 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     lib.sfa_attn_decode_window.restype = ctypes.c_int
     lib.sfa_prefill_window_workspace_bytes.argtypes = [D, i32, i32, i32, i32]
     lib.sfa_prefill_window_workspace_bytes.restype = size
+    lib.sfa_prefill_window_workspace_bound.argtypes = [D, i32]
+    lib.sfa_prefill_window_workspace_bound.restype = size
     lib.sfa_attn_prefill_window.argtypes = [D, P, P, P, i32, i32, i32, i32, i32, f32, P, size, P]
     lib.sfa_attn_prefill_window.restype = ctypes.c_int
     _lib = lib
@@ -220,10 +223,12 @@ SFA_ATTEND_WINDOW = 1
 #: every symbol include/sfa_pager.h declares
 HOST_EXPORTS = (
     "sfa_pager_create",
+    "sfa_pager_create_sinks",
     "sfa_pager_destroy",
     "sfa_pager_begin",
     "sfa_pager_append",
     "sfa_pager_rope_append",
+    "sfa_pager_norm_rope_append",
     "sfa_pager_attend",
     "sfa_pager_append_attend",
     "sfa_pager_reset",
@@ -282,6 +287,11 @@ def load_host(path: Path | str | None = None) -> ctypes.CDLL:
     i32 = ctypes.c_int32
     lib.sfa_pager_create.argtypes = [ctypes.POINTER(SfaPagerConfig), ctypes.POINTER(P)]
     lib.sfa_pager_create.restype = ctypes.c_int
+    lib.sfa_pager_create_sinks.argtypes = [ctypes.POINTER(SfaPagerConfig), i32, ctypes.POINTER(P)]
+    lib.sfa_pager_create_sinks.restype = ctypes.c_int
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    lib.sfa_pager_norm_rope_append.argtypes = [P, i32, ctypes.POINTER(SfaRopeDesc), P, i64, P, P, i64, P, i64, P, P, f32, P, P]
+    lib.sfa_pager_norm_rope_append.restype = ctypes.c_int
     lib.sfa_pager_destroy.argtypes = [P]
     lib.sfa_pager_destroy.restype = None
     lib.sfa_pager_begin.argtypes = [P, P, P]

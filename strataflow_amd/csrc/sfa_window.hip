@@ -36,6 +36,9 @@ static int window_args(const sfa_kv_desc *kv, const float *q, float *out, const 
     p->window = window;
     p->n_sink = n_sink;
     p->scale_log2 = scale * 1.44269504088896340736f;
+    if (!__builtin_isfinite(p->scale_log2)) return SFA_ERR_INVALID_ARGUMENT;
+    // a tile's offsets are 32-bit, with room for those under its first row
+    if ((int64_t)p->row_bytes * kv->n_head_kv * 64 > (1 << 30)) return SFA_ERR_UNSUPPORTED;
     return SFA_OK;
 }
 
@@ -93,6 +96,11 @@ SFA_API size_t sfa_prefill_window_workspace_bytes(const sfa_kv_desc *kv, int32_t
         return 0;
     const int n = sfa::window_prefill_splits(kv, q_pos0, T, window, n_sink);
     return n == 1 ? 0 : sfa::records_bytes((int64_t)T * kv->n_head, n, kv->head_dim);
+}
+
+SFA_API size_t sfa_prefill_window_workspace_bound(const sfa_kv_desc *kv, int32_t max_T) {
+    if (sfa_kv_desc_check(kv) != SFA_OK || max_T <= 0) return 0;
+    return sfa::records_bytes(sfa::window_prefill_most_records(kv, max_T), 2, kv->head_dim) / 2;
 }
 
 SFA_API int sfa_attn_prefill_window(const sfa_kv_desc *kv, const float *q, float *out,

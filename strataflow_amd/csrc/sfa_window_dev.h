@@ -34,6 +34,7 @@ struct WindowParams {
 int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink);
 int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s);
 int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int32_t window, int32_t n_sink);
+int64_t window_prefill_most_records(const sfa_kv_desc *kv, int32_t max_T);
 int window_prefill_launch(const WindowParams &p, const sfa_kv_desc *kv, hipStream_t s);
 int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipStream_t s);
 

@@ -19,7 +19,9 @@
 
 namespace sfa {
 
-constexpr int kRows = 128;  // of a workgroup
+constexpr int kRows = 128;         // of a workgroup
+constexpr int kMostSplits = 64;    // of a row block's tiles
+constexpr int kMostBlocks = 1024;  // workgroups where there are splits
 
 template <int KVT, int HD>
 struct PTile {
@@ -717,7 +719,7 @@ int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int3
     const double record = 2.0 * T * kv->n_head * kv->head_dim * 4 / 3.5e6;
     int best = 1;
     double least = 0.0;
-    for (int n = 1; n <= 64 && n <= tiles && (n == 1 || blocks * n <= 1024); ++n) {
+    for (int n = 1; n <= kMostSplits && n <= tiles && (n == 1 || blocks * n <= kMostBlocks); ++n) {
         const int64_t cu = (blocks * n + 255) / 256;
         const double us = (double)((tiles + n - 1) / n) * tile * (cu == 1 ? 1.0 : pair * cu / 2) + (n > 1 ? 3.0 + n * record : 0.0);
         if (n == 1 || us < least) {
@@ -726,6 +728,20 @@ int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int3
         }
     }
     return best;
+}
+
+// The most (row, split) records that a call of up to max_T tokens may write.
+int64_t window_prefill_most_records(const sfa_kv_desc *kv, int32_t max_T) {
+    const int g = kv->n_head / kv->n_head_kv;
+    int64_t most = 0;
+    // the splits allowed fall where a row block is added: the last T of a block count
+    for (int64_t block = 1;; ++block) {
+        const int64_t T = block * kRows / g < max_T ? block * kRows / g : max_T;
+        int64_t n = kMostBlocks / (block * kv->n_head_kv);
+        n = n > kMostSplits ? kMostSplits : n;
+        if (n > 1 && T * kv->n_head * n > most) most = T * kv->n_head * n;
+        if (n <= 1 || T == max_T) return most;
+    }
 }
 
 template <int KVT, int HD>

@@ -26,6 +26,7 @@
 #include "page_planner.h"
 #include "sfa.h"
 #include "sfa_pager.h"
+#include "sfa_window.h"
 
 namespace {
 
@@ -75,6 +76,7 @@ struct sfa_pager {
     size_t page_bytes = 0;
     int max_pages = 0;
     int32_t max_span = 0;
+    int32_t n_sink = -1;           // sfa_pager_create_sinks; -1: one window for a step
     uint8_t *dev_pool = nullptr;   // [layer][K|V][n_pages][page_bytes]
     uint8_t *cold_pool = nullptr;  // [layer][K|V][n_cold][page_bytes], host-pinned
     int32_t *d_table = nullptr;    // [n_seq][max_pages]
@@ -97,10 +99,11 @@ struct sfa_pager {
     bool step_open = false;
     int64_t bytes_evicted = 0;
 
-    sfa_pager(const sfa_pager_config &c, int n_pages, int n_cold)
+    sfa_pager(const sfa_pager_config &c, int n_pages, int n_cold, int32_t sinks)
         : cfg(c),
           planner(c.n_seq, c.page_size, (uint32_t)c.n_ctx, (uint32_t)c.window, n_pages, n_cold,
-                  c.attend == SFA_ATTEND_LOSSLESS, c.seed, /*async_evict=*/true) {}
+                  c.attend == SFA_ATTEND_LOSSLESS, c.seed, /*async_evict=*/true, sinks),
+          n_sink(sinks) {}
 
     ~sfa_pager() {
         for (auto &e : ev_flight) (void)hipEventDestroy(e.second);
@@ -227,9 +230,8 @@ struct sfa_pager {
     }
 };
 
-extern "C" {
-
-SFA_API int sfa_pager_create(const sfa_pager_config *cfg_in, sfa_pager **out) {
+// sfa_pager_create, or with n_sink >= 0 sfa_pager_create_sinks.
+static int create(const sfa_pager_config *cfg_in, int32_t n_sink, sfa_pager **out) {
     if (cfg_in == nullptr || out == nullptr) return SFA_ERR_INVALID_ARGUMENT;
     *out = nullptr;
     sfa_pager_config c = *cfg_in;
@@ -243,6 +245,11 @@ SFA_API int sfa_pager_create(const sfa_pager_config *cfg_in, sfa_pager **out) {
     if (c.window == 0 || c.window > c.n_ctx) c.window = c.n_ctx;
     const int max_pages = (c.n_ctx + c.page_size - 1) / c.page_size;
     const int win_pages = (c.window + c.page_size - 1) / c.page_size + 1;
+    if (c.n_pages <= 0 && n_sink >= 0) {
+        // a step's tokens see window - 1 + n_tok positions of the window, and the sinks
+        const int64_t P = c.page_size, kept = ((int64_t)c.window + P - 2) / P + 2 + ((int64_t)n_sink + P - 1) / P;
+        c.n_pages = c.n_seq * (int)std::min<int64_t>(kept, max_pages);
+    }
     if (c.n_pages <= 0) c.n_pages = c.n_seq * std::min(win_pages, max_pages);
     const bool paging = c.window < c.n_ctx;
     if (c.attend == SFA_ATTEND_LOSSLESS && paging) {
@@ -262,7 +269,7 @@ SFA_API int sfa_pager_create(const sfa_pager_config *cfg_in, sfa_pager **out) {
 
     sfa_pager *p = nullptr;
     try {
-        p = new sfa_pager(c, c.n_pages, c.n_cold_pages);
+        p = new sfa_pager(c, c.n_pages, c.n_cold_pages, n_sink);
         p->page_bytes = sfa_page_bytes(&d);
         p->max_pages = max_pages;
         p->max_span = c.attend == SFA_ATTEND_WINDOW ? c.window : c.n_ctx;
@@ -311,6 +318,9 @@ SFA_API int sfa_pager_create(const sfa_pager_config *cfg_in, sfa_pager **out) {
         }
     }
     p->ws_bytes = sfa_decode_workspace_bytes(&p->descs[0], c.n_seq, p->max_span);
+    if (n_sink >= 0)
+        p->ws_bytes = std::max(sfa_decode_window_workspace_bytes(&p->descs[0], c.n_seq, c.n_ctx, c.window, n_sink),
+                               sfa_prefill_window_workspace_bound(&p->descs[0], c.page_size));
     if (p->ws_bytes == 0) return fail(SFA_ERR_INVALID_ARGUMENT);
     if (hipMalloc(&p->ws, p->ws_bytes) != hipSuccess) return fail(SFA_ERR_OUT_OF_MEMORY);
     // default-priority copy stream and the step marker of deferred eviction
@@ -321,6 +331,17 @@ SFA_API int sfa_pager_create(const sfa_pager_config *cfg_in, sfa_pager **out) {
     if (hipDeviceSynchronize() != hipSuccess) return fail(SFA_ERR_RUNTIME);
     *out = p;
     return SFA_OK;
+}
+
+extern "C" {
+
+SFA_API int sfa_pager_create(const sfa_pager_config *cfg, sfa_pager **out) { return create(cfg, -1, out); }
+
+SFA_API int sfa_pager_create_sinks(const sfa_pager_config *cfg, int32_t n_sink, sfa_pager **out) {
+    if (out != nullptr) *out = nullptr;
+    if (cfg == nullptr || n_sink < 0 || cfg->attend != SFA_ATTEND_WINDOW || cfg->window <= 0)
+        return SFA_ERR_INVALID_ARGUMENT;
+    return create(cfg, n_sink, out);
 }
 
 SFA_API void sfa_pager_destroy(sfa_pager *p) {
@@ -401,6 +422,35 @@ SFA_API int sfa_pager_rope_append(sfa_pager *p, int32_t layer, float *q, const f
                               p->d_table, p->max_pages, freq_base, stream);
 }
 
+SFA_API int sfa_pager_norm_rope_append(sfa_pager *p, int32_t layer, const sfa_rope_desc *rope, const float *q,
+                                       int64_t q_stride, float *q_out, const float *k, int64_t k_stride,
+                                       const float *v, int64_t v_stride, const float *q_norm, const float *k_norm,
+                                       float eps, const int32_t *rope_pos, void *stream) {
+    if (p == nullptr || !p->step_open || layer < 0 || layer >= p->cfg.n_layer)
+        return SFA_ERR_INVALID_ARGUMENT;
+    return sfa_norm_rope_kv_append(&p->descs[layer], rope, q, q_stride, q_out, k, k_stride, v, v_stride, q_norm, k_norm,
+                                   eps, p->d_tok_seq, p->d_tok_pos, rope_pos, p->step_tokens, p->d_table, p->max_pages,
+                                   stream);
+}
+
+// Attention of a step under a window for every token and the sinks.
+static int attend_sinks(sfa_pager *p, const sfa_kv_desc *d, const float *q, float *out, bool one_each, float scale,
+                        void *stream) {
+    if (one_each)
+        return sfa_attn_decode_window(d, q, out, p->d_table, p->max_pages, p->d_seq_len, p->cfg.window, p->n_sink,
+                                      p->cfg.n_seq, p->cfg.n_ctx, scale, p->ws, p->ws_bytes, stream);
+    const size_t row = (size_t)p->cfg.n_head * p->cfg.head_dim;
+    for (int b = 0; b < p->cfg.n_seq; ++b) {
+        if (p->step_ntok[b] == 0) continue;
+        const size_t off = (size_t)p->step_off[b] * row;
+        const int rc = sfa_attn_prefill_window(d, q + off, out + off, p->d_table + (size_t)b * p->max_pages,
+                                               p->max_pages, p->step_pos0[b], p->step_ntok[b], p->cfg.window, p->n_sink,
+                                               scale, p->ws, p->ws_bytes, stream);
+        if (rc != SFA_OK) return rc;
+    }
+    return SFA_OK;
+}
+
 SFA_API int sfa_pager_attend(sfa_pager *p, int32_t layer, const float *q, float *out,
                              void *stream) {
     if (p == nullptr || !p->step_open || layer < 0 || layer >= p->cfg.n_layer)
@@ -410,6 +460,7 @@ SFA_API int sfa_pager_attend(sfa_pager *p, int32_t layer, const float *q, float 
     const bool windowed = p->cfg.attend == SFA_ATTEND_WINDOW;
     const bool one_each = std::all_of(p->step_ntok.begin(), p->step_ntok.end(),
                                       [](int32_t n) { return n == 1; });
+    if (p->n_sink >= 0) return attend_sinks(p, d, q, out, one_each, scale, stream);
     if (one_each)
         return sfa_attn_decode(d, q, out, p->d_table, p->max_pages, p->d_seq_len,
                                windowed ? p->d_kv_lo : nullptr, p->cfg.n_seq, p->max_span, scale,
@@ -438,7 +489,7 @@ SFA_API int sfa_pager_append_attend(sfa_pager *p, int32_t layer, const float *k,
         return SFA_ERR_INVALID_ARGUMENT;
     const bool one_each = std::all_of(p->step_ntok.begin(), p->step_ntok.end(),
                                       [](int32_t n) { return n == 1; });
-    if (!one_each || p->cfg.kv_type == SFA_KV_Q8_0) {
+    if (!one_each || p->cfg.kv_type == SFA_KV_Q8_0 || p->n_sink >= 0) {
         const int rc = sfa_pager_append(p, layer, k, v, stream);
         return rc != SFA_OK ? rc : sfa_pager_attend(p, layer, q, out, stream);
     }

@@ -20,11 +20,13 @@ bool KvStore::evicts(uint32_t pos, uint32_t *evicted) const {
 }
 
 PagePlanner::PagePlanner(int n_seq, int page_size, uint32_t n_ctx, uint32_t window, int n_pages,
-                         int n_cold_pages, bool keep_cold, uint64_t seed, bool async_evict)
+                         int n_cold_pages, bool keep_cold, uint64_t seed, bool async_evict, int n_sink)
     : page_size_(page_size),
       max_pages_((int)((n_ctx + (uint32_t)page_size - 1) / (uint32_t)page_size)),
       keep_cold_(keep_cold),
       async_(async_evict && keep_cold),
+      n_sink_(keep_cold ? -1 : n_sink),
+      drop_next_(n_seq, 0),
       rng_(seed) {
     stores_.reserve(n_seq);
     for (int b = 0; b < n_seq; ++b) stores_.emplace_back(n_ctx, 0, window);
@@ -92,8 +94,48 @@ uint32_t PagePlanner::attend_lo(int seq) const {
     return pos + 1 > st.window() ? pos + 1 - st.window() : 0;
 }
 
+void PagePlanner::allocate(int seq, int32_t lpage, std::vector<PageAction> *actions) {
+    const int32_t dev = take_device_page(actions);
+    actions->push_back({PageAction::kAlloc, seq, lpage, dev, -1, 0, false, true});
+    table_[(std::size_t)seq * max_pages_ + lpage] = dev;
+    ++stats_.allocated;
+    ++stats_.dev_in_use;
+}
+
+int PagePlanner::plan_sinks(int seq, int n_tok, std::vector<PageAction> *actions) {
+    KvStore &st = stores_[seq];
+    if (!st.can_fit((uint32_t)n_tok)) return 1;
+    const int64_t P = page_size_, pos0 = st.used(), W = st.window();
+    int32_t *row = &table_[(std::size_t)seq * max_pages_];
+    // the step's first token, at pos0, sees positions > pos0 - W and the sinks
+    int32_t end = drop_next_[seq];
+    int64_t dev_free = (int64_t)free_dev_.size();
+    while ((end + 1) * P <= pos0 - W + 1) {
+        if (end * P >= n_sink_ && row[end] >= 0) ++dev_free;
+        ++end;
+    }
+    if (n_tok > 0)
+        for (int64_t lp = pos0 / P; lp <= (pos0 + n_tok - 1) / P; ++lp)
+            if (row[lp] == -1 && --dev_free < 0) return 4;
+    for (int32_t lp = drop_next_[seq]; lp < end; ++lp) {
+        if (lp * P < n_sink_ || row[lp] < 0) continue;
+        actions->push_back({PageAction::kDrop, seq, lp, row[lp], -1, 0, false, true});
+        free_dev_.push_back(row[lp]);
+        row[lp] = -1;
+        ++stats_.dropped;
+        --stats_.dev_in_use;
+    }
+    drop_next_[seq] = end;
+    if (n_tok > 0)
+        for (int64_t lp = pos0 / P; lp <= (pos0 + n_tok - 1) / P; ++lp)
+            if (row[lp] == -1) allocate(seq, (int32_t)lp, actions);
+    st.advance((uint32_t)n_tok);
+    return 0;
+}
+
 int PagePlanner::plan(int seq, int n_tok, std::vector<PageAction> *actions) {
     if (seq < 0 || seq >= (int)stores_.size() || n_tok < 0 || n_tok > page_size_) return 1;
+    if (n_sink_ >= 0) return plan_sinks(seq, n_tok, actions);
     KvStore &st = stores_[seq];
     if (!st.can_fit((uint32_t)n_tok)) return 1;
     const uint32_t P = (uint32_t)page_size_;
@@ -146,13 +188,7 @@ int PagePlanner::plan(int seq, int n_tok, std::vector<PageAction> *actions) {
                 --stats_.dev_in_use;
             }
         }
-        if (pos % P == 0 && row[pos / P] == -1) {
-            const int32_t dev = take_device_page(actions);
-            actions->push_back({PageAction::kAlloc, seq, (int32_t)(pos / P), dev, -1, 0, false, true});
-            row[pos / P] = dev;
-            ++stats_.allocated;
-            ++stats_.dev_in_use;
-        }
+        if (pos % P == 0 && row[pos / P] == -1) allocate(seq, (int32_t)(pos / P), actions);
     }
     st.advance((uint32_t)n_tok);
     return 0;
@@ -208,6 +244,7 @@ void PagePlanner::reset(int seq, std::vector<PageAction> *actions) {
         row[lp] = -1;
     }
     stores_[seq].reset();
+    drop_next_[seq] = 0;
 }
 
 }  // namespace sfa

@@ -80,8 +80,12 @@ public:
     // keep_cold: lossless (evicted pages go to the cold pool) vs sliding window
     // (evicted pages are dropped).  A sequence holds at most
     // ceil(window / page_size) + 1 device pages.
+    // n_sink >= 0 (keep_cold false): a window for every token of a step, and the
+    // first n_sink positions stay.  A page is dropped at the first step none of
+    // whose tokens sees it, before the step's pages are allocated; pages with
+    // positions under n_sink never are.
     PagePlanner(int n_seq, int page_size, uint32_t n_ctx, uint32_t window, int n_pages,
-                int n_cold_pages, bool keep_cold, uint64_t seed, bool async_evict = false);
+                int n_cold_pages, bool keep_cold, uint64_t seed, bool async_evict = false, int n_sink = -1);
 
     // Plans writing positions [used, used + n_tok) of sequence `seq`, in order,
     // and advances its KvStore.  n_tok <= page_size.  Returns 0 or an sf_status
@@ -126,6 +130,8 @@ private:
     int32_t take_cold_page();
     uint64_t next_random();
     void retire_front(bool wait, std::vector<PageAction> *actions);
+    int plan_sinks(int seq, int n_tok, std::vector<PageAction> *actions);
+    void allocate(int seq, int32_t lpage, std::vector<PageAction> *actions);
 
     int page_size_;
     int max_pages_;
@@ -135,6 +141,8 @@ private:
     std::vector<Pending> pending_;  // evictions in flight, oldest first
     std::vector<KvStore> stores_;
     std::vector<int32_t> table_;
+    int n_sink_;                     // -1: one window for a step, no sinks
+    std::vector<int32_t> drop_next_;  // with sinks: the first page not yet looked at for dropping
     std::vector<int32_t> free_dev_;
     std::vector<int32_t> free_cold_;
     uint64_t rng_;

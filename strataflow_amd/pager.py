@@ -28,13 +28,18 @@ class KvPager:
     def __init__(self, *, n_layer: int, n_head: int, n_head_kv: int, head_dim: int, kv_type: int,
                  page_size: int, n_seq: int, n_ctx: int, window: int = 0,
                  attend: int = SFA_ATTEND_LOSSLESS, n_pages: int = 0, n_cold_pages: int = 0,
-                 seed: int = 0):
+                 seed: int = 0, n_sink: int | None = None):
+        """n_sink: a windowed model's pager (sfa_pager_create_sinks): a window for
+        every token, and the first n_sink positions stay visible."""
         self._h = None
         lib = _lib.load_host()
         c = _lib.SfaPagerConfig(n_layer, n_head, n_head_kv, head_dim, kv_type, page_size, n_seq,
                                 n_ctx, window, attend, n_pages, n_cold_pages, seed)
         h = ctypes.c_void_p()
-        _lib.check(lib.sfa_pager_create(ctypes.byref(c), ctypes.byref(h)), "sfa_pager_create")
+        if n_sink is None:
+            _lib.check(lib.sfa_pager_create(ctypes.byref(c), ctypes.byref(h)), "sfa_pager_create")
+        else:
+            _lib.check(lib.sfa_pager_create_sinks(ctypes.byref(c), n_sink, ctypes.byref(h)), "sfa_pager_create_sinks")
         self._h = h
         self.n_layer, self.n_head, self.n_head_kv, self.head_dim = n_layer, n_head, n_head_kv, head_dim
         self.n_seq, self.n_ctx, self.page_size, self.attend_mode = n_seq, n_ctx, page_size, attend
@@ -83,6 +88,32 @@ class KvPager:
         _lib.check(_lib.load_host().sfa_pager_rope_append(
             self._h, layer, None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
             float(freq_base), _stream()), "sfa_pager_rope_append")
+
+    def norm_rope_append(self, layer: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                         rope: _lib.SfaRopeDesc, q_norm: torch.Tensor | None = None,
+                         k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                         rope_pos: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Head norms, rotation and append (PagedKV.norm_rope_append): q [n_tok,
+        Hq, hd] (or None), k, v [n_tok, Hkv, hd] f32, slices of stacked rows
+        allowed; returns the rotated Q."""
+        n, hd = self.n_tokens, self.head_dim
+        dev = k.device
+        for t, heads in ((q, self.n_head), (k, self.n_head_kv), (v, self.n_head_kv)):
+            if t is not None and (t.dtype is not torch.float32 or not t.is_cuda or t.device != dev or t.shape != (n, heads, hd)
+                                  or t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
+                raise ValueError(f"q, k and v must be float32 [{n}, heads, {hd}], a token's heads one after the other")
+        for w in (q_norm, k_norm):
+            if w is not None and (w.dtype is not torch.float32 or w.device != dev or w.shape != (hd,) or not w.is_contiguous()):
+                raise ValueError(f"norms must be contiguous float32 [{hd}]")
+        if rope_pos is not None and (rope_pos.dtype is not torch.int32 or rope_pos.device != dev
+                                     or rope_pos.shape != (rope.n_axis, n) or not rope_pos.is_contiguous()):
+            raise ValueError(f"rope_pos must be contiguous int32 [{rope.n_axis}, {n}]")
+        out = None if q is None else q.new_empty((n, self.n_head, hd))
+        ptr = lambda t: None if t is None else t.data_ptr()
+        _lib.check(_lib.load_host().sfa_pager_norm_rope_append(
+            self._h, layer, rope, ptr(q), 0 if q is None else q.stride(0), ptr(out), k.data_ptr(), k.stride(0), v.data_ptr(),
+            v.stride(0), ptr(q_norm), ptr(k_norm), float(eps), ptr(rope_pos), _stream()), "sfa_pager_norm_rope_append")
+        return out
 
     def attend(self, layer: int, q: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         assert q.is_contiguous() and q.dtype == torch.float32

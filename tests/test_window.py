@@ -119,3 +119,79 @@ def test_workspace_sizes():
     assert lib.sfa_decode_window_workspace_bytes(desc(), 2, MAX, 64, 4) <= lib.sfa_decode_window_workspace_bytes(desc(), 2, MAX, MAX, MAX) < 1 << 30
     for bad in ((-1, 5, 64, 4), (0, 0, 64, 4), (0, 5, 0, 4), (0, 5, 64, -1), (MAX, 5, 64, 4)):
         assert lib.sfa_prefill_window_workspace_bytes(desc(), *bad) == 0
+    # the bound covers every call of up to so many tokens
+    import random
+    rng = random.Random(0)
+    for _ in range(3000):
+        g = rng.choice([1, 2, 4, 8])
+        hkv = rng.choice([1, 2, 3, 8, 16, 64])
+        kv = desc(n_head=g * hkv, n_head_kv=hkv, kv_type=rng.choice([0, 1, 8]), head_dim=rng.choice([64, 128]))
+        T = rng.randint(1, rng.choice([4, 64, 1000, 9000]))
+        need = lib.sfa_prefill_window_workspace_bytes(kv, rng.randint(0, 100000), T, rng.randint(1, 20000), rng.randint(0, 300))
+        assert need <= lib.sfa_prefill_window_workspace_bound(kv, T)
+        assert lib.sfa_prefill_window_workspace_bound(kv, T) <= lib.sfa_prefill_window_workspace_bound(kv, T + 77)
+    assert lib.sfa_prefill_window_workspace_bound(desc(), 0) == 0
+
+
+def test_prefill_needs_its_workspace():
+    need = _lib.load().sfa_prefill_window_workspace_bytes(desc(), 20000, 93, 4096, 4)
+    assert need > 0
+    assert prefill(pos0=20000, T=93, window=4096, ws=None) == BAD
+    assert prefill(pos0=20000, T=93, window=4096, size=need - 1) == BAD
+    assert prefill(pos0=20000, T=93, window=4096, ws=P + 64) == UNS
+
+
+def test_rows_past_32_bit_tiles_are_refused():
+    assert decode(kv=desc(n_head=1 << 20, n_head_kv=1 << 20)) == UNS
+    assert prefill(kv=desc(n_head=1 << 20, n_head_kv=1 << 20)) == UNS
+
+
+def test_python_refusals():
+    """What the wrapper checks before a pointer is passed on (on the host: tensors without a GPU)."""
+    import torch
+
+    from strataflow_amd.paged_kv import PagedKV
+    kv = PagedKV(1, 8, 2, 64, _lib.SFA_KV_F16, 64, 2, device="cpu")
+    q, i = torch.zeros(2, 8, 64), torch.zeros(2, dtype=torch.int32)
+    for bad in (q.double(), q[:, :4], q.transpose(0, 1).contiguous(), torch.zeros(2, 8, 128)[..., :64]):
+        with pytest.raises(ValueError):
+            kv._rows(bad, None, 2, None)
+    with pytest.raises(ValueError):
+        kv._rows(q, torch.zeros(2, 511), 2, None)
+    x = torch.zeros(2, 12, 64)
+    assert kv._heads(x[:, 8:10], "k", 2, 2) == 12 * 64
+    for bad in (x[:, 8:10].double(), x[:, 8:11], x[:, ::6], x.transpose(0, 1)[:2, :2]):
+        with pytest.raises(ValueError):
+            kv._heads(bad, "k", 2, 2)
+    assert i.numel() == 2
+
+
+def test_pager_create_refusals():
+    lib = _lib.load_host()
+    c = _lib.SfaPagerConfig(1, 8, 2, 64, _lib.SFA_KV_F16, 64, 1, 256, 128, _lib.SFA_ATTEND_WINDOW, 0, 0, 0)
+    h = ctypes.c_void_p(1)
+
+    def create(n_sink, **kw):
+        d = _lib.SfaPagerConfig.from_buffer_copy(c)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return lib.sfa_pager_create_sinks(ctypes.byref(d), n_sink, ctypes.byref(h))
+
+    assert create(-1) == BAD and h.value is None
+    assert create(4, attend=_lib.SFA_ATTEND_LOSSLESS) == BAD
+    assert create(4, window=0) == BAD
+    assert create(4, page_size=96) == UNS
+    assert lib.sfa_pager_create_sinks(None, 4, ctypes.byref(h)) == BAD
+    assert lib.sfa_pager_create_sinks(ctypes.byref(c), 4, None) == BAD
+    assert lib.sfa_pager_norm_rope_append(None, 0, None, None, 0, None, None, 0, None, 0, None, None, 1e-6, None, None) == BAD
+
+
+def test_page_planner_sinks_cpp(tmp_path):
+    import subprocess
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    host, exe = root / "strataflow_amd" / "host", tmp_path / "page_planner_sinks_test"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", f"-I{host}", str(root / "tests" / "cpp" / "page_planner_sinks_test.cpp"),
+                    str(host / "page_planner.cpp"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert out.startswith("ok ") and int(out.split()[1]) > 1000
