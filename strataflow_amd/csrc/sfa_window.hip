@@ -29,6 +29,7 @@ static int window_args(const sfa_kv_desc *kv, const float *q, float *out, const 
     p->n_pages = kv->n_pages;
     p->n_cold = kv->n_cold_pages;
     p->page_size = kv->page_size;
+    p->page_shift = (kv->page_size & (kv->page_size - 1)) == 0 ? __builtin_ctz((unsigned)kv->page_size) : -1;
     p->max_pages = max_pages;
     p->n_head = kv->n_head;
     p->n_head_kv = kv->n_head_kv;

@@ -70,10 +70,14 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
     // in one L2 (8 sequences, window 8192: the step 59 -> 51 us).  Whole lines are
     // faster from all over the chip (F16, 64 sequences: 190 us against 200).
     constexpr bool kShared = KVT == SFA_KV_Q8_0;
-    const int kvh = (kShared ? blockIdx.x / 8 : blockIdx.x) % p.n_head_kv;
-    const int part = kShared ? blockIdx.x / (8 * p.n_head_kv) * 8 + blockIdx.x % 8 : blockIdx.x / p.n_head_kv;
-    const int split = part % p.n_split, b = part / p.n_split;
-    if (b >= p.n_tok) return;  // (the parts of a Q8_0 cache are rounded up to eight)
+    int kvh = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
+    if constexpr (kShared) {
+        kvh = blockIdx.y;
+        const int part = blockIdx.z * 8 + blockIdx.x;
+        b = (int)to_scalar((uint32_t)part / (uint32_t)p.n_split);
+        split = part - b * p.n_split;
+        if (b >= p.n_tok) return;  // (the parts are rounded up to eight)
+    }
     const int32_t *table = p.page_table + (int64_t)b * p.max_pages;
     const int len = p.seq_len[b];
 
@@ -104,8 +108,8 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
     const int ns = min(min(p.n_sink, lo), hi + 1);
     const int sink_tiles = pos < 0 ? 0 : (ns + TP - 1) / TP;
     const int n_tiles = pos < 0 ? 0 : sink_tiles + (hi >= lo ? hi / TP - lo / TP + 1 : 0);
-    const int t0 = (int)((int64_t)n_tiles * split / p.n_split);
-    const int t1 = (int)((int64_t)n_tiles * (split + 1) / p.n_split);
+    int t0, t1;
+    split_range(n_tiles, split, p.n_split, t0, t1);
 
     const int col_bytes = p.n_head_kv * T::RB;
     int k_off[T::NI], v_off[T::NI];
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
         const bool sink = t < sink_tiles;
         const int first = (sink ? t : lo / TP + t - sink_tiles) * TP;
         const int from = max(sink ? 0 : lo - first, 0), to = min((sink ? ns : hi + 1) - first, TP);
-        const int lp = first / p.page_size;
+        const int lp = page_of(p, first);
         const int32_t id = pages.get(table, p.max_pages, lp, lane);
         const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
         const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
     };
     int t = t0 + wave;
     if (t < t1) {
-        pages.load(table, p.max_pages, (t < sink_tiles ? t * TP : (lo / TP + t - sink_tiles) * TP) / p.page_size, lane);
+        pages.load(table, p.max_pages, page_of(p, (t < sink_tiles ? t : lo / TP + t - sink_tiles) * TP), lane);
         issue(t, 0);
     }
 
@@ -509,18 +513,18 @@ int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, 
 }
 
 template <int KVT, int HD>
-static void launch_g(const WindowParams &p, unsigned grid, hipStream_t s) {
+static void launch_g(const WindowParams &p, dim3 grid, hipStream_t s) {
     const dim3 block(64 * kWaves);
     switch (p.n_head / p.n_head_kv) {
-    case 1: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 1>), dim3(grid), block, 0, s, p); break;
-    case 2: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 2>), dim3(grid), block, 0, s, p); break;
-    case 4: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 4>), dim3(grid), block, 0, s, p); break;
-    default: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 8>), dim3(grid), block, 0, s, p); break;
+    case 1: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 1>), grid, block, 0, s, p); break;
+    case 2: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 2>), grid, block, 0, s, p); break;
+    case 4: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 4>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((window_decode_kernel<KVT, HD, 8>), grid, block, 0, s, p); break;
     }
 }
 
 template <int KVT>
-static int launch_hd(const WindowParams &p, int head_dim, unsigned grid, hipStream_t s) {
+static int launch_hd(const WindowParams &p, int head_dim, dim3 grid, hipStream_t s) {
     if (head_dim == 128) launch_g<KVT, 128>(p, grid, s);
     else if (head_dim == 64) launch_g<KVT, 64>(p, grid, s);
     else if constexpr (KVT != SFA_KV_Q8_0) launch_g<KVT, 32>(p, grid, s);
@@ -529,14 +533,15 @@ static int launch_hd(const WindowParams &p, int head_dim, unsigned grid, hipStre
 }
 
 int window_decode_launch(const WindowParams &p, const sfa_kv_desc *kv, int32_t B, hipStream_t s) {
-    const int64_t parts = (int64_t)B * p.n_split;
-    const int64_t grid = (kv->kv_type == SFA_KV_Q8_0 ? (parts + 7) / 8 * 8 : parts) * kv->n_head_kv, rows = (int64_t)B * kv->n_head;
-    if (grid > INT32_MAX || rows > INT32_MAX) return SFA_ERR_UNSUPPORTED;
+    const int64_t rows = (int64_t)B * kv->n_head;
+    if (B > 65535 || kv->n_head_kv > 65535 || rows > INT32_MAX) return SFA_ERR_UNSUPPORTED;
+    const dim3 grid = kv->kv_type == SFA_KV_Q8_0 ? dim3(8, (unsigned)kv->n_head_kv, (unsigned)(((int64_t)B * p.n_split + 7) / 8))
+                                                 : dim3((unsigned)kv->n_head_kv, (unsigned)p.n_split, (unsigned)B);
     int rc;
     switch (kv->kv_type) {
-    case SFA_KV_F32: rc = launch_hd<SFA_KV_F32>(p, kv->head_dim, (unsigned)grid, s); break;
-    case SFA_KV_F16: rc = launch_hd<SFA_KV_F16>(p, kv->head_dim, (unsigned)grid, s); break;
-    case SFA_KV_Q8_0: rc = launch_hd<SFA_KV_Q8_0>(p, kv->head_dim, (unsigned)grid, s); break;
+    case SFA_KV_F32: rc = launch_hd<SFA_KV_F32>(p, kv->head_dim, grid, s); break;
+    case SFA_KV_F16: rc = launch_hd<SFA_KV_F16>(p, kv->head_dim, grid, s); break;
+    case SFA_KV_Q8_0: rc = launch_hd<SFA_KV_Q8_0>(p, kv->head_dim, grid, s); break;
     default: return SFA_ERR_UNSUPPORTED;
     }
     if (rc != SFA_OK || p.n_split == 1) return rc;

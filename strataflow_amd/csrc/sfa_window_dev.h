@@ -19,6 +19,7 @@ struct WindowParams {
     const uint8_t *k_pages, *v_pages, *k_cold, *v_cold;
     int64_t page_bytes;
     int n_pages, n_cold, page_size, max_pages;
+    int page_shift;          // log2(page_size), -1 where there is none
     int n_head, n_head_kv, row_bytes;
     const int32_t *page_table;
     const int32_t *seq_len;  // decode; null for a chunk
@@ -45,6 +46,19 @@ int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipSt
 __device__ inline uint32_t to_scalar(uint32_t x) {
     asm("" : "+v"(x));
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+
+// The tiles of a split: n / splits, and one more for the first n % splits.
+// (Divisions run on the vector side: back to scalars, for scalar branches.)
+__device__ inline void split_range(int n, int split, int splits, int &t0, int &t1) {
+    const int each = (int)to_scalar((uint32_t)n / (uint32_t)splits), more = n - each * splits;
+    t0 = split * each + min(split, more);
+    t1 = t0 + each + (split < more ? 1 : 0);
+}
+
+// Logical page of a position.
+__device__ inline int page_of(const WindowParams &p, int pos) {
+    return p.page_shift >= 0 ? pos >> p.page_shift : (int)to_scalar((uint32_t)pos / (uint32_t)p.page_size);
 }
 
 // A raw buffer over [base, base + bytes): loads outside it give zeros, also

@@ -98,9 +98,7 @@ __device__ inline Block block_of(const WindowParams &p, int wave, int n) {
     b.ns = min(min(p.n_sink, b.lo), b.hi + 1);
     b.sink_tiles = (b.ns + TP - 1) / TP;
     const int n_tiles = b.sink_tiles + (b.hi >= b.lo ? b.hi / TP - b.lo / TP + 1 : 0);
-    // (the divisions run on the vector side: back to scalars, for scalar branches)
-    b.t0 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * b.split / p.n_split));
-    b.t1 = (int)to_scalar((uint32_t)((uint64_t)n_tiles * (b.split + 1) / p.n_split));
+    split_range(n_tiles, b.split, p.n_split, b.t0, b.t1);
     return b;
 }
 
@@ -119,7 +117,7 @@ __device__ inline Src source(const WindowParams &p, const Block &b, PageWindow &
     s.first = (s.sink ? t : b.lo / TP + t - b.sink_tiles) * TP;
     s.from = max(s.sink ? 0 : b.lo - s.first, 0);
     s.to = min((s.sink ? b.ns : b.hi + 1) - s.first, TP);
-    const int lp = (int)to_scalar((uint32_t)s.first / (uint32_t)p.page_size);
+    const int lp = page_of(p, s.first);
     const int32_t id = pages.get(p.page_table, p.max_pages, lp, lane);
     const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
     const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
@@ -138,7 +136,7 @@ template <int TP>
 __device__ inline void page_window(const WindowParams &p, const Block &b, PageWindow &pages, int lane) {
     const int t = b.t0;
     if (t < b.t1)
-        pages.load(p.page_table, p.max_pages, (t < b.sink_tiles ? t : b.lo / TP + t - b.sink_tiles) * TP / p.page_size, lane);
+        pages.load(p.page_table, p.max_pages, page_of(p, (t < b.sink_tiles ? t : b.lo / TP + t - b.sink_tiles) * TP), lane);
 }
 
 // Whether the token at tpos sees row r of a tile.
@@ -176,27 +174,24 @@ __device__ inline void look_over(uint8_t *v, uint8_t *bits_of, uint64_t *bad, in
 
 __device__ inline bool any_bad(const uint64_t *bad) { return __ballot((bad[0] | bad[1] | bad[2] | bad[3]) != 0) != 0; }
 
-// NaN to the outputs of the lane's row that a value set to zero has a part in;
-// was(r, e): whether V's value e of row r was.
-template <int HD, typename O, typename Was>
-__device__ inline void spoil(const WindowParams &p, const Src &s, int tpos, int hh, O &o, Was was) {
-    asm("" : "+v"(hh));  // (its 16 multiples are not held over the loop)
+// The lane's outputs that a value set to zero has a part in, a bit for each
+// o[d][i] at 16 d + i; was(r, e): whether V's value e of row r was.  A small loop
+// that leaves o alone: it hardly ever runs, and the registers are full.
+template <int HD, typename Was>
+__device__ inline uint64_t spoiled(const WindowParams &p, const Src &s, int tpos, int hh, Was was) {
+    uint64_t bits = 0;
     for (int r = s.from; r < s.to; ++r) {
-        const bool see = sees(p, s, r, tpos);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int e = 32 * d + i / 4 * 8 + 4 * hh + i % 4;  // the dim of o[d][i]
-                o[d][i] = (was(r, e) & see) ? NAN : o[d][i];
-                if (i % 4 == 3) asm volatile("" ::: "memory");  // few reads at a time
-            }
+        if (!sees(p, s, r, tpos)) continue;
+#pragma unroll 1
+        for (int j = 0; j < HD / 2; ++j)
+            bits |= (uint64_t)was(r, j / 16 * 32 + j % 16 / 4 * 8 + 4 * hh + j % 4) << j;
     }
+    return bits;
 }
 
-// The lane's outputs, or its split record.
+// The lane's outputs, NaN where a bit of `bad` is set, or its split record.
 template <int HD, typename O>
-__device__ inline void store_row(const WindowParams &p, const Block &b, int hh, const O &o, float base, float l, float unit) {
+__device__ inline void store_row(const WindowParams &p, const Block &b, int hh, const O &o, float base, float l, float unit, uint64_t bad) {
     if (!b.row_ok) return;
     float la, lb;
     swap_halves(l, la, lb);
@@ -210,7 +205,7 @@ __device__ inline void store_row(const WindowParams &p, const Block &b, int hh, 
         for (int i4 = 0; i4 < 4; ++i4) {
             floatx4 x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = o[d][4 * i4 + i] * w;
+            for (int i = 0; i < 4; ++i) x[i] = bad >> (16 * d + 4 * i4 + i) & 1 ? NAN : o[d][4 * i4 + i] * w;
             *reinterpret_cast<floatx4 *>(dst + 32 * d + 8 * i4 + 4 * hh) = x;
         }
     if (p.n_split > 1 && hh == 0) p.rec_ml[row * p.n_split + b.split] = make_float2(base, l);
@@ -290,6 +285,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
     // probabilities are 2^(s f - base), base kSplitShift below the row's running
     // maximum; l sums this lane's
     float base = -INFINITY, l = 0.0f;
+    uint64_t bad = 0;
     floatx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -368,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
                                   o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[st], o[d], 0, 0, 0);
                               });
         if (src.masked && any_bad(v_bad[par]))
-            spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int e) { return (bool)(v_bits[par][r * T::CPR + pv_slot<HD>(r, e / 8)] >> e % 8 & 1); });
+            bad |= spoiled<HD>(p, src, b.tpos, hh, [&](int r, int e) { return v_bits[par][r * T::CPR + pv_slot<HD>(r, e / 8)] >> e % 8 & 1; });
     };
 
     Src cur = {}, next = {};
@@ -387,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
         if (t + 1 < b.t1) next = issue(t + 1, par ^ 1);
         if (b.wave_ok && cur.there) tile(cur, par);
     }
-    store_row<HD>(p, b, hh, o, base, l, 1.0f);
+    store_row<HD>(p, b, hh, o, base, l, 1.0f, bad);
 }
 
 // The F32 and Q8_0 kernel: caches whose values are wider than an f16.  A tile
@@ -549,6 +545,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
     // maximum; l sums this lane's; o is in units of 2^(unit_exp - 127 - V_SHIFT),
     // unit_exp the exponent of the largest of V so far
     float base = -INFINITY, l = 0.0f;
+    uint64_t bad = 0;
     int unit_exp = 1;
     floatx16 o[DB];
 #pragma unroll
@@ -582,7 +579,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
         if constexpr (!kQ8) {
-            pipelined<KC, 2, FENCE>(
+            pipelined<KC, 1, FENCE>(
                 [&](int c) {
                     const uint8_t *const at = &lds[0][0] + (k_at ^ (32 * c));
                     return Two{*reinterpret_cast<const half8 *>(at), *reinterpret_cast<const half8 *>(at + T::BYTES)};
@@ -601,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
         } else {
             // two steps a block, then the block's scales
             floatx16 x;
-            pipelined<KC * PB, 3, FENCE>(
+            pipelined<KC * PB, 2, FENCE>(
                 [&](int i) {
                     const int blk = i / 2 % PB, c = i / (2 * PB) * 2 + i % 2;
                     return *reinterpret_cast<const half8 *>(&lds[0][0] + (k_at ^ (32 * c)) + blk * 32 * T::ROW);
@@ -676,7 +673,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
             const half4 x = tr16_read(at), y = tr16_read(at + 8 * T::ROW);
             return half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         };
-        pipelined<ST * DB, 2, FENCE>([&](int i) { return Two{v_read(SETS - 2, i / DB, i % DB), v_read(SETS - 1, i / DB, i % DB)}; },
+        pipelined<ST * DB, 1, FENCE>([&](int i) { return Two{v_read(SETS - 2, i / DB, i % DB), v_read(SETS - 1, i / DB, i % DB)}; },
                                      [&](int i, Two a) {
                                          const int st = i / DB, d = i % DB;
                                          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hi, ph[st], o[d], 0, 0, 0);
@@ -687,19 +684,19 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
             // units of V: NB / 2 * 128 of them in the waves that hold V
             constexpr int W0 = NB == 4 ? 0 : 2;
             if (__ballot((v_bad[W0] | v_bad[W0 + 1] | v_bad[2] | v_bad[3]) != 0) != 0)
-                spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int d) {
-                    const int u = r * NB + d / kQK;
-                    return (bool)(v_bad[W0 + u / 64] >> u % 64 & 1);
+                bad |= spoiled<HD>(p, src, b.tpos, hh, [&](int r, int e) {
+                    const int u = r * NB + e / kQK;
+                    return v_bad[W0 + u / 64] >> u % 64 & 1;
                 });
         } else {
             if (any_bad(v_bad))
-                spoil<HD>(p, src, b.tpos, hh, o, [&](int r, int d) {
-                    const int th = r * 8 + d / FPT;
-                    return (bool)((v_bad[th / 64] >> th % 64 & 1) & (v_bits[th] >> d % FPT & 1));
+                bad |= spoiled<HD>(p, src, b.tpos, hh, [&](int r, int e) {
+                    const int th = r * 8 + e / FPT;
+                    return (v_bad[th / 64] >> th % 64 & 1) & (v_bits[th] >> e % FPT & 1);
                 });
         }
     }
-    store_row<HD>(p, b, hh, o, base, l, __builtin_amdgcn_ldexpf(1.0f, unit_exp - 127 - V_SHIFT));
+    store_row<HD>(p, b, hh, o, base, l, __builtin_amdgcn_ldexpf(1.0f, unit_exp - 127 - V_SHIFT), bad);
 }
 
 // Workgroups that share a row block's tiles: the number with the least estimated
