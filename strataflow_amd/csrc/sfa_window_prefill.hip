@@ -35,8 +35,10 @@ struct PTile {
     static constexpr int NG = ROW / 64 > 0 ? ROW / 64 : 1;
 };
 
-// Where chunk j of row r lies in its LDS row: K's reads are 16 rows at one
-// chunk, V's four rows at 64 neighbouring bytes.
+// Where chunk j of row r lies in its LDS row.  K's reads are 16 rows at one
+// chunk, V's four rows at 64 neighbouring bytes; writes of Q8_0 and F32 rows
+// are one chunk of every block of neighbouring rows: all of these fall in
+// different banks.
 template <int HD>
 __device__ inline int pk_slot(int r, int j) {
     using T = PTile<SFA_KV_F16, HD>;
@@ -45,7 +47,8 @@ __device__ inline int pk_slot(int r, int j) {
 template <int HD>
 __device__ inline int pv_slot(int r, int j) {
     using T = PTile<SFA_KV_F16, HD>;
-    return j ^ (r / T::RP % T::NG * 4);
+    const int q = r / T::RP;
+    return j ^ (q % T::NG * 4) ^ (q % (HD == 32 ? 2 : 4));
 }
 
 // Runs the N steps of a product loop with the operand reads AHEAD steps before
