@@ -79,7 +79,7 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
         if (b >= p.n_tok) return;  // (the parts are rounded up to eight)
     }
     const int32_t *table = p.page_table + (int64_t)b * p.max_pages;
-    const int len = p.seq_len[b];
+    const int len = max(p.seq_len[b], 0);
 
     // Q of column c: rows past G are zero columns
     float amax = 0.0f;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
     const int lo = pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
     const int hi = pos < cap ? pos : (int)(cap - 1);
     const int ns = min(min(p.n_sink, lo), hi + 1);
-    const int sink_tiles = pos < 0 ? 0 : (ns + TP - 1) / TP;
+    const int sink_tiles = pos < 0 ? 0 : tiles_of(ns, TP);
     const int n_tiles = pos < 0 ? 0 : sink_tiles + (hi >= lo ? hi / TP - lo / TP + 1 : 0);
     int t0, t1;
     split_range(n_tiles, split, p.n_split, t0, t1);
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                 ql[ks][j] = l;
             }
     }
-    const float f = p.scale_log2 * up;
+    const float f = KVT == SFA_KV_F32 ? p.scale_log2 : score_factor(p.scale_log2, up);
 
     // probabilities are 2^(s f - base), base kSplitShift below the column's
     // running maximum (F32: at it); l sums this lane's

@@ -56,6 +56,14 @@ __device__ inline void split_range(int n, int split, int splits, int &t0, int &t
     t1 = t0 + each + (split < more ? 1 : 0);
 }
 
+// Tiles of n positions from a tile's first one (n up to INT32_MAX).
+__device__ inline int tiles_of(int n, int tp) { return n / tp + (n % tp != 0); }
+
+// Factor of the scores in the exponent of two, under a row's power of two
+// (row_exponent).  Never zero: a masked score stays -inf.  (Where it would be,
+// the row's scores differ by less than 2^-80.)
+__device__ inline float score_factor(float scale_log2, float up) { return fmaxf(scale_log2 * up, 0x1p-126f); }
+
 // Logical page of a position.
 __device__ inline int page_of(const WindowParams &p, int pos) {
     return p.page_shift >= 0 ? pos >> p.page_shift : (int)to_scalar((uint32_t)pos / (uint32_t)p.page_size);

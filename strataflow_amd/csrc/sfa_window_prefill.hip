@@ -99,7 +99,7 @@ __device__ inline Block block_of(const WindowParams &p, int wave, int n) {
     b.lo = b.first - p.window + 1 > 0 ? b.first - p.window + 1 : 0;
     b.hi = b.last < cap ? b.last : (int)(cap - 1);
     b.ns = min(min(p.n_sink, b.lo), b.hi + 1);
-    b.sink_tiles = (b.ns + TP - 1) / TP;
+    b.sink_tiles = tiles_of(b.ns, TP);
     const int n_tiles = b.sink_tiles + (b.hi >= b.lo ? b.hi / TP - b.lo / TP + 1 : 0);
     split_range(n_tiles, b.split, p.n_split, b.t0, b.t1);
     return b;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
     page_window<TP>(p, b, pages, lane);
 
     half8 qh[KC], ql[KC];
-    const float f = p.scale_log2 * split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql);
+    const float f = score_factor(p.scale_log2, split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql));
 
     // This wave's quarter of a tile, lane by lane: load i has RPI rows more than
     // load 0, which flips bit 2 of K's slots i times and leaves V's (few registers:
@@ -419,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
     PageWindow pages;
     page_window<TP>(p, b, pages, lane);
     half8 qh[KC], ql[KC];
-    const float f = p.scale_log2 * split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql);
+    const float f = score_factor(p.scale_log2, split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql));
 
     // What a thread brings of a tile.  F32: 1/8 of a row of K and of V.  Q8_0: a
     // block; with HD 128 one of K and one of V, with HD 64 the first two waves
