@@ -18,7 +18,12 @@
  * sfa_attn_prefill the attentions here round neither Q nor a probability to 16
  * bits: over an F16 or Q8_0 cache a 32-bit factor goes through the matrix
  * cores as two f16 halves, so that outputs are those of 32-bit arithmetic on
- * the values that the cache holds (relative error of some 1e-6).
+ * the values that the cache holds (relative error of some 1e-6).  Over an F32
+ * cache K and V beyond 2^90 may overflow on the way.
+ *
+ * NaN and infinities: what a token may not see has no part in its row.  Of
+ * what it sees, a NaN in K makes the head's outputs NaN, one in V those of its
+ * element (Q8_0: of the block with such a scale); an infinity may do the same.
  */
 #ifndef SFA_WINDOW_H
 #define SFA_WINDOW_H
@@ -69,7 +74,7 @@ SFA_API int sfa_rope_desc_check(const sfa_rope_desc *rope, int32_t head_dim);
  *             NULL for `pos` on every axis
  * A token with seq < 0 or pos < 0 is skipped (its q_out row is not written); one
  * whose page is not there has its Q written only.  Where two tokens name the
- * same position, which one stays is not defined.
+ * same position, what that row then holds is not defined.
  * q, q_out, k and v 16-byte aligned, strides multiples of 4 that hold a
  * token's heads (one token: any); else SFA_ERR_UNSUPPORTED, or
  * SFA_ERR_INVALID_ARGUMENT for a stride that is too small. */
@@ -93,8 +98,9 @@ SFA_API size_t sfa_decode_window_workspace_bytes(const sfa_kv_desc *kv, int32_t 
  * whose pages is there, gets zeros; positions past the table or on a page that
  * is not there are not attended, and pages outside the window and the sinks are
  * not read, so their entries may be -1.
- * q and out 16-byte aligned and the workspace 256-byte aligned (else
- * SFA_ERR_UNSUPPORTED).  Calls that overlap in time need a workspace each; its
+ * q and out 16-byte aligned and the workspace 256-byte aligned, B and n_head_kv
+ * at most 65535, 64 positions of a tensor in at most 1 GiB (else
+ * SFA_ERR_UNSUPPORTED).  scale > 0, and scale * log2(e) finite.  Calls that overlap in time need a workspace each; its
  * contents before a call do not matter. */
 SFA_API int sfa_attn_decode_window(const sfa_kv_desc *kv, const float *q, float *out,
                                    const int32_t *page_table, int32_t max_pages,
@@ -117,10 +123,9 @@ SFA_API size_t sfa_prefill_window_workspace_bound(const sfa_kv_desc *kv, int32_t
  * positions p <= t with p < n_sink or p > t - window.  q, out, page_table,
  * max_pages, scale as sfa_attn_prefill; q_pos0 + T must not pass INT32_MAX.
  * Positions past the table or on a page that is not there are not attended; a
- * token that so attends nothing gets zeros.  What a token may not see has no
- * part in its row, NaN and infinities included.  page_size must be a
- * multiple of 64 (SFA_ERR_UNSUPPORTED otherwise); alignment and workspace as
- * sfa_attn_decode_window. */
+ * token that so attends nothing gets zeros.  page_size must be a multiple of 64
+ * and T * n_head / n_head_kv at most 65535 * 128 (SFA_ERR_UNSUPPORTED
+ * otherwise); alignment, scale and workspace as sfa_attn_decode_window. */
 SFA_API int sfa_attn_prefill_window(const sfa_kv_desc *kv, const float *q, float *out,
                                     const int32_t *page_table, int32_t max_pages, int32_t q_pos0,
                                     int32_t T, int32_t window, int32_t n_sink, float scale,

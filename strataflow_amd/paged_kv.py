@@ -61,6 +61,9 @@ def _stream(stream) -> int:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+_INT32_MAX = 2 ** 31 - 1  # what is larger would be taken modulo 2^32
+
+
 def _raw_stream(stream, device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else _stream(stream)
 
@@ -362,6 +365,8 @@ class PagedKV:
         if (page_table.dtype is not i32 or page_table.get_device() != dev or page_table.dim() != 2
                 or page_table.shape[0] != B or not page_table.is_contiguous()):
             raise self._bad("page_table", "int32", f"[{B}, max_pages]")
+        if max(max_seq_len, window, n_sink) > _INT32_MAX:
+            raise ValueError("max_seq_len, window and n_sink are 32-bit")
         lib, d = _lib.load(), self._descs[layer]
         key = (B, max_seq_len, window, n_sink)
         need = self._ws_window.get(key)
@@ -391,6 +396,8 @@ class PagedKV:
         out = self._rows(q, out, T, stream)
         if page_table.dtype is not torch.int32 or page_table.get_device() != dev or page_table.dim() != 1 or not page_table.is_contiguous():
             raise self._bad("page_table", "int32", "[max_pages]")
+        if max(q_pos0, window, n_sink) > _INT32_MAX:
+            raise ValueError("q_pos0, window and n_sink are 32-bit")
         lib, d = _lib.load(), self._descs[layer]
         need = lib.sfa_prefill_window_workspace_bytes(d, q_pos0, T, window, n_sink)
         ws = _empty((need,), out, stream, torch.uint8) if need else None

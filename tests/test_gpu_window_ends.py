@@ -53,3 +53,14 @@ def test_lengths_at_both_ends(gpu, kv_type):
     table[0, 1] = -1
     got = c.kv.decode_window(0, cuda(q[:1]), table, lens, INT_MAX, 1, INT_MAX)
     check(got, *c.attend(0, q[:1], [INT_MAX - 1], 1, INT_MAX), 64)
+
+
+def test_arguments_past_32_bits(gpu):
+    c = Cache(lens=[64], n_head=2, n_head_kv=2, head_dim=64, page_size=64, seed=7)
+    q, lens = cuda(c.queries(1)), torch.tensor([64], dtype=torch.int32).cuda()
+    for more in ((2 ** 32 + 64, 8, 0), (64, 2 ** 32 + 8, 0), (64, 8, 2 ** 31)):
+        with pytest.raises(ValueError):
+            c.kv.decode_window(0, q, c.t_table, lens, *more)
+    for more in ((2 ** 32 + 63, 8, 0), (63, 2 ** 32 + 8, 0), (63, 8, 2 ** 31)):
+        with pytest.raises(ValueError):
+            c.kv.prefill_window(0, q, c.t_table[0], *more)

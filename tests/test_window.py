@@ -109,6 +109,17 @@ def test_descriptor_refusals():
     assert decode(kv=desc(page_size=32), B=0) == OK
 
 
+def test_limits_of_a_launch():
+    """What a grid or a 32-bit offset cannot hold is refused, not cut."""
+    size = 1 << 44
+    many = desc(n_head=1, n_head_kv=1)
+    assert decode(kv=many, B=65536, size=size) == UNS
+    assert prefill(kv=many, T=65535 * 128 + 1, size=size) == UNS
+    wide = desc(kv_type=_lib.SFA_KV_F32, head_dim=128, n_head=32769, n_head_kv=32769, page_size=64)
+    assert decode(kv=wide, size=size) == UNS and prefill(kv=wide, size=size) == UNS
+    assert decode(scale=3e38) == BAD and prefill(scale=3e38) == BAD  # times log2(e) it is no f32
+
+
 def test_workspace_sizes():
     lib = _lib.load()
     for bad in ((0, 500, 64, 4), (2, 0, 64, 4), (2, 500, 0, 4), (2, 500, 64, -1)):
