@@ -338,11 +338,13 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                 for (int mt = 0; mt < MT; ++mt) {
                     const floatx4 d = *reinterpret_cast<const floatx4 *>(tab + nb * TP + 16 * mt + 4 * qd);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        _Float16 h, lo16;
-                        split_f16(pr[mt][i] * d[i], h, lo16);
-                        ph[4 * mt + i] = h;
-                        pl[4 * mt + i] = lo16;
+                    for (int i = 0; i < 4; i += 2) {
+                        half2v h, lo16;
+                        float u = pr[mt][i] * d[i], v = pr[mt][i + 1] * d[i + 1];
+                        asm("" : "+v"(u), "+v"(v));  // (see split_f16)
+                        split2_f16(u, v, h, lo16);
+                        ph[4 * mt + i] = h[0], ph[4 * mt + i + 1] = h[1];
+                        pl[4 * mt + i] = lo16[0], pl[4 * mt + i + 1] = lo16[1];
                     }
                 }
                 // rows of two products: dims 2 c and 2 c + 1 of the block, one 16-bit read a position

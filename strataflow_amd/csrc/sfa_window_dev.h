@@ -160,16 +160,22 @@ __device__ inline void row_exponent(float amax, float &down, float &up) {
 }
 
 // Quants as f16 (exact): byte b is 1024 + (b + 128) under the exponent of 1024.
-__device__ inline half2v quants2(uint32_t two) {  // bytes 0 and 2
+__device__ inline half2v quants2(uint32_t two) {  // bytes 0 and 2, the others 0
     const half2v base = {(_Float16)1152.0f, (_Float16)1152.0f};
     return __builtin_bit_cast(half2v, two ^ 0x64806480u) - base;
 }
 __device__ inline half8 quants8(uint32_t a, uint32_t b) {
+    const half2v base = {(_Float16)1152.0f, (_Float16)1152.0f};
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    const uint32_t w[4] = {__builtin_amdgcn_perm(0x64646464u, a, 0x04010400), __builtin_amdgcn_perm(0x64646464u, a, 0x04030402),
+                           __builtin_amdgcn_perm(0x64646464u, b, 0x04010400), __builtin_amdgcn_perm(0x64646464u, b, 0x04030402)};
     half8 r;
-    const half2v h[4] = {quants2(__builtin_amdgcn_perm(0, a, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, a, 0x0c030c02)),
-                         quants2(__builtin_amdgcn_perm(0, b, 0x0c010c00)), quants2(__builtin_amdgcn_perm(0, b, 0x0c030c02))};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[2 * i] = h[i][0], r[2 * i + 1] = h[i][1];
+    for (int i = 0; i < 4; ++i) {
+        const half2v h = __builtin_bit_cast(half2v, w[i]) - base;
+        r[2 * i] = h[0], r[2 * i + 1] = h[1];
+    }
     return r;
 }
 

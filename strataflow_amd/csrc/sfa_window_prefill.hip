@@ -350,9 +350,10 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const int e = 8 * st + j;
-                const float u = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], f, -sub));
-                const float v = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16 + 1], f, -sub));
+                float u = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16], f, -sub));
+                float v = __builtin_amdgcn_exp2f(fmaf(s[e / 16][e % 16 + 1], f, -sub));
                 l += u + v;
+                asm("" : "+v"(u), "+v"(v) : "v"(l));
                 half2v h, r;
                 split2_f16(u, v, h, r);
                 ph[st][j] = h[0], ph[st][j + 1] = h[1];
