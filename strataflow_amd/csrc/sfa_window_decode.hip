@@ -3,10 +3,17 @@
 //
 // Bound by memory: a sequence's visible K and V rows are read once.  They are
 // cut into tiles of 4 KB to 8 KB a tensor; a wave streams its tiles through
-// two LDS buffers of its own (asynchronous loads, the next tile under way
-// while one is computed), with the running maximum and sum of the softmax, and
-// the waves of a workgroup, then the workgroups of a sequence (the merge
-// kernel), join their (maximum, sum, output).
+// LDS of its own, with the running maximum and sum of the softmax.  The next
+// K is under way from the end of the first product on and the next V from the
+// end of the second, so that one buffer each does and LDS has room for twice
+// the waves that two would leave (Q8_0, 8 sequences, window 8192, with append
+// and merge: 49 -> 47 us; one F16 token 12.2 -> 12.0).  The waves of a
+// workgroup, then the workgroups of a sequence (the merge kernel), join their
+// (maximum, sum, output).
+//
+// Measured (32 / 8 heads of 128): F16, 64 sequences, window 4096: 185 us, 5.8
+// TB/s.  Q8_0, 8 sequences, window 8192: 37 us of kernel, 3.9 TB/s; its loads
+// alone take 33 (rows of 136 bytes), its arithmetic alone 28.
 //
 // S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions: their 16 columns
 // are the G query heads of a kv head, and lane l holds column l % 16 of both,
@@ -50,15 +57,19 @@ __device__ inline int v_slot(int r, int j) {
     return j;
 }
 
+// Workgroups of a CU: as many as LDS holds, but for Q8_0 of HD 128: a fourth
+// would leave too few registers.
+template <int KVT, int HD>
+constexpr int kGroups = HD != 128 ? 4 : KVT == SFA_KV_Q8_0 ? 3 : 2;
+
 template <int KVT, int HD, int G>
-__global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 2) void window_decode_kernel(WindowParams p) {
+__global__ __launch_bounds__(64 * kWaves, (kGroups<KVT, HD>)) void window_decode_kernel(WindowParams p) {
     using T = Tile<KVT, HD>;
     constexpr int TP = T::TP, MT = TP / 16;  // 16-position blocks of a tile
     constexpr int KS = HD / 32, DB = HD / 16;
     constexpr int NB = HD / kQK;             // quantisation blocks of a row
-    constexpr int STAGE = 2 * T::BYTES;
     constexpr int TAB = KVT == SFA_KV_Q8_0 ? 2 * NB * TP * 4 : 0;  // a wave's scales of the tile, K and V
-    constexpr int WAVE = 2 * STAGE + TAB;
+    constexpr int WAVE = 2 * T::BYTES + TAB;
     constexpr int JOIN = (int)sizeof(float) * kWaves * G * (HD + 2);
     __shared__ __attribute__((aligned(256))) uint8_t lds[kWaves * WAVE > JOIN ? kWaves * WAVE : JOIN];
 
@@ -122,39 +133,47 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
     uint8_t *const mine = lds + wave * WAVE;
     const uint32_t mine_at = lds_addr(mine);
     PageWindow pages;
-    int r0[2], r1[2];  // visible rows of the tile in each buffer
-    auto issue = [&](int t, int buf) {
+    // A tile: its first visible rows in the pools, their bytes, and which rows of
+    // the tile they are.  The buffer holds the visible rows alone: what else the
+    // tile's place in the page holds is not read.
+    struct Src {
+        const uint8_t *k, *v;
+        int bytes, back, from, to;
+    };
+    auto source = [&](int t) {
         const bool sink = t < sink_tiles;
         const int first = (sink ? t : lo / TP + t - sink_tiles) * TP;
-        const int from = max(sink ? 0 : lo - first, 0), to = min((sink ? ns : hi + 1) - first, TP);
+        Src s;
+        s.from = max(sink ? 0 : lo - first, 0);
+        s.to = min((sink ? ns : hi + 1) - first, TP);
         const int lp = page_of(p, first);
         const int32_t id = pages.get(table, p.max_pages, lp, lane);
         const uint8_t *kb = page_base(id, p.k_pages, p.n_pages, p.k_cold, p.n_cold, p.page_bytes);
         const uint8_t *vb = page_base(id, p.v_pages, p.n_pages, p.v_cold, p.n_cold, p.page_bytes);
         const bool there = kb != nullptr && vb != nullptr;
-        // the buffer holds the visible rows alone: what else the tile's place in
-        // the page holds is not read
-        const int64_t row = (int64_t)(first - lp * p.page_size + from) * col_bytes + kvh * T::RB;
-        const int bytes = there ? (to - from - 1) * col_bytes + T::RB : 0;
-        const auto kr = buffer_of(there ? kb + row : nullptr, bytes);
-        const auto vr = buffer_of(there ? vb + row : nullptr, bytes);
-        const int up = from * col_bytes;
-        const uint32_t at = mine_at + buf * STAGE;
-        // (the last instruction of Q8_0 by the lanes that have a chunk left)
-        constexpr int LAST = TP * T::CPR - 64 * (T::NI - 1);
-#pragma unroll
-        for (int i = 0; i < T::NI; ++i)
-            if (i < T::NI - 1 || LAST == 64 || lane < LAST) load_to_lds(kr, at + 1024 * i, k_off[i] - up);
-#pragma unroll
-        for (int i = 0; i < T::NI; ++i)
-            if (i < T::NI - 1 || LAST == 64 || lane < LAST) load_to_lds(vr, at + T::BYTES + 1024 * i, v_off[i] - up);
-        r0[buf] = from;
-        r1[buf] = there ? to : 0;
+        const int64_t row = (int64_t)(first - lp * p.page_size + s.from) * col_bytes + kvh * T::RB;
+        s.k = there ? kb + row : nullptr;
+        s.v = there ? vb + row : nullptr;
+        s.bytes = there ? (s.to - s.from - 1) * col_bytes + T::RB : 0;
+        s.back = s.from * col_bytes;
+        if (!there) s.to = 0;
+        return s;
     };
+    // (the last instruction of Q8_0 by the lanes that have a chunk left)
+    constexpr int LAST = TP * T::CPR - 64 * (T::NI - 1);
+    auto load = [&](const uint8_t *rows, const Src &s, const int (&off)[T::NI], uint32_t at) {
+        const auto r = buffer_of(rows, s.bytes);
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i)
+            if (i < T::NI - 1 || LAST == 64 || lane < LAST) load_to_lds(r, at + 1024 * i, off[i] - s.back);
+    };
+    Src cur = {}, next = {};
     int t = t0 + wave;
     if (t < t1) {
         pages.load(table, p.max_pages, page_of(p, (t < sink_tiles ? t : lo / TP + t - sink_tiles) * TP), lane);
-        issue(t, 0);
+        cur = source(t);
+        load(cur.k, cur, k_off, mine_at);
+        load(cur.v, cur, v_off, mine_at + T::BYTES);
     }
 
     // Q as two f16 under a power of two of its row, or as it is
@@ -190,17 +209,10 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    int buf = 0;
-    for (; t < t1; t += kWaves, buf ^= 1) {
-        // the reads of this buffer's last tile are done before it is filled again
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (t + kWaves < t1) {
-            issue(t + kWaves, buf ^ 1);
-            wait_loads<2 * T::NI>();
-        } else {
-            wait_loads<0>();
-        }
-        const uint8_t *const ks0 = mine + buf * STAGE, *const vs0 = ks0 + T::BYTES;
+    const uint8_t *const ks0 = mine, *const vs0 = mine + T::BYTES;
+    for (; t < t1; t += kWaves, cur = next) {
+        const bool more = t + kWaves < t1;
+        wait_loads<T::NI>();  // K is there
         floatx4 s[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s[mt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -223,27 +235,14 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                     s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], qx[ks / 2][ks % 2 * 4 + i], s[0], 0, 0, 0);
             }
         } else {
-            // the blocks' scales, K then V, as f32 [block][position]: a lane needs those of its
-            // eight score rows, whose K rows are other lanes' operands
-            float *const tab = reinterpret_cast<float *>(mine + 2 * STAGE);
-            const int tp = lane & 31;
-            const uint8_t *const src = (lane < 32 ? ks0 : vs0) + tp * T::ROW;
-            float d[NB], dmax = 0.0f;
+            // the blocks' scales as f32 [block][position]: a lane needs those of its eight
+            // score rows, whose K rows are other lanes' operands
+            float *const tab = reinterpret_cast<float *>(mine + 2 * T::BYTES);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                d[nb] = (float)*reinterpret_cast<const _Float16 *>(src + kQ8Bytes * nb);
-                dmax = fmaxf(dmax, fabsf(d[nb]));
+            for (int i = 0; i < NB / 2; ++i) {
+                const int nb = NB / 2 * (lane >> 5) + i;
+                tab[nb * TP + (lane & 31)] = (float)*reinterpret_cast<const _Float16 *>(ks0 + (lane & 31) * T::ROW + kQ8Bytes * nb);
             }
-            const int e = max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, wave_max(lane < 32 ? 0.0f : dmax)) >> 23)), 1);
-            if (e > unit) {
-                const float a = __builtin_amdgcn_ldexpf(1.0f, unit - e);
-#pragma unroll
-                for (int i = 0; i < DB; ++i) o[i] *= a;
-                unit = e;
-            }
-            const float down = lane < 32 ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, 127 - unit);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) tab[(lane < 32 ? 0 : NB * TP) + nb * TP + tp] = d[nb] * down;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -267,7 +266,13 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                     for (int i = 0; i < 4; ++i) s[mt][i] = fmaf(x[i], d[i], s[mt][i]);
                 }
         }
-        const int from = r0[buf], to = r1[buf];
+        // K's reads are done: the next tile's
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            next = source(t + kWaves);
+            load(next.k, next, k_off, mine_at);
+        }
+        const int from = cur.from, to = cur.to;
         if (from > 0 || to < TP) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -299,6 +304,9 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                 pr[mt][i] = __builtin_amdgcn_exp2f(fmaf(s[mt][i], f, -sub));
                 l += pr[mt][i];
             }
+        // V is there
+        if (more) wait_loads<T::NI>();
+        else wait_loads<0>();
         if constexpr (KVT == SFA_KV_F32) {
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -329,7 +337,24 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[d], 0, 0, 0);
             }
         } else {
-            const float *const tab = reinterpret_cast<const float *>(mine + 2 * STAGE) + NB * TP;
+            float *const tab = reinterpret_cast<float *>(mine + 2 * T::BYTES) + NB * TP;
+            float d[NB / 2], dmax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i) {
+                d[i] = (float)*reinterpret_cast<const _Float16 *>(vs0 + (lane & 31) * T::ROW + kQ8Bytes * (NB / 2 * (lane >> 5) + i));
+                dmax = fmaxf(dmax, fabsf(d[i]));
+            }
+            const int e = max(__builtin_amdgcn_readfirstlane((int)(__builtin_bit_cast(uint32_t, wave_max(dmax)) >> 23)), 1);
+            if (e > unit) {
+                const float a = __builtin_amdgcn_ldexpf(1.0f, unit - e);
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[i] *= a;
+                unit = e;
+            }
+            const float down = __builtin_amdgcn_ldexpf(1.0f, 127 - unit);
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i) tab[(NB / 2 * (lane >> 5) + i) * TP + (lane & 31)] = d[i] * down;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 // a position's block scale goes with its probability
@@ -369,6 +394,10 @@ __global__ __launch_bounds__(64 * kWaves, KVT != SFA_KV_Q8_0 && HD == 128 ? 1 : 
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load(next.v, next, v_off, mine_at + T::BYTES);
         }
     }
 
@@ -501,9 +530,12 @@ int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipSt
     return hipGetLastError() == hipSuccess ? SFA_OK : SFA_ERR_RUNTIME;
 }
 
-// Workgroups of one sequence and kv head: as many as fill the chip once (one
-// workgroup a CU where its buffers take over half the LDS, else two), at most
-// one per four tiles of the longest span.
+// Workgroups of one sequence and kv head: as many as give every CU one (F16
+// and F32 of HD 128) or two, at most one per four tiles of the longest span.
+// More records cost more than a fuller chip gives: F16, one sequence, window
+// 4096 (32 / 8 heads of 128): 12.2 / 11.5 / 12.0 / 12.5 us with 16 / 24 / 32 /
+// 48; 64 sequences 182 / 193 with 1 / 2; Q8_0, 8 sequences, window 8192: 53 /
+// 46.4 / 46.5 / 48.7 with 4 / 8 / 12 / 16.
 int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink) {
     const int tp = kv->kv_type == SFA_KV_F32 ? 16 : 32;
     const int64_t seen = (int64_t)window + n_sink < max_seq_len ? (int64_t)window + n_sink : max_seq_len;
