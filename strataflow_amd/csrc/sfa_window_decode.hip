@@ -536,9 +536,17 @@ int window_merge_launch(const WindowParams &p, int head_dim, int64_t rows, hipSt
 // 4096 (32 / 8 heads of 128): 12.2 / 11.5 / 12.0 / 12.5 us with 16 / 24 / 32 /
 // 48; 64 sequences 182 / 193 with 1 / 2; Q8_0, 8 sequences, window 8192: 53 /
 // 46.4 / 46.5 / 48.7 with 4 / 8 / 12 / 16.
+// Short spans stay with one, whose rounds of a tile a wave take `round` us each,
+// against a second launch: 2 us, and 2.7 more where the host issues every call.
+// Measured (two sequences; one workgroup / split, GPU alone): F16, heads of
+// 128: window 124 6.5 / 7.2, 252 7.7 / 7.6, 508 9.9 / 7.7; Q8_0 124 8.7 / 8.5,
+// 252 10.9 / 8.7; F32 heads of 32: 252 6.7 / 6.4, 508 10.0 / 6.6.
 int window_decode_splits(const sfa_kv_desc *kv, int32_t B, int32_t max_seq_len, int32_t window, int32_t n_sink) {
-    const int tp = kv->kv_type == SFA_KV_F32 ? 16 : 32;
+    const bool f32 = kv->kv_type == SFA_KV_F32, f16 = kv->kv_type == SFA_KV_F16;
+    const int tp = f32 ? 16 : 32;
     const int64_t seen = (int64_t)window + n_sink < max_seq_len ? (int64_t)window + n_sink : max_seq_len;
+    const double width = kv->head_dim / 128.0, round = f32 ? 0.3 + 1.5 * width : f16 ? 0.6 + 0.55 * width : 1.1 + 1.1 * width;
+    if (((double)seen / (tp * kWaves) - 1.0) * round <= 2.1) return 1;
     const int64_t tiles = (seen + tp - 1) / tp + 2;
     const int64_t room = kv->head_dim == 128 && kv->kv_type != SFA_KV_Q8_0 ? 256 : 512;
     int64_t n = room / ((int64_t)B * kv->n_head_kv);
