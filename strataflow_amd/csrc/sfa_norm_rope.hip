@@ -8,6 +8,10 @@
 // Bound by memory: Q is read and written, K and V read (f32), their rows written.
 // A lane owns 8 elements of a head, four whole pairs, so that a rotation
 // needs no other lane; the sum of squares joins the HD/8 lanes of a head by DPP.
+// A token's angles are computed once, in 64 bits, for all its heads.
+// Measured (32 / 8 heads of 128): 8192 tokens into an F32 cache 80 us, 5.0 TB/s
+// (a large copy: 5.15); 2048 into F16 17.4 us, 5.3 TB/s; one token 4 us, the
+// chain of its position, its page and its row.
 #include "sfa_append.h"
 #include "sfa_window.h"
 
@@ -195,10 +199,11 @@ static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 template <int KVT>
 static int launch_hd(const NormRopeParams &p, hipStream_t s) {
-    // few tokens: a workgroup for every 256 lanes' heads, each with its own table
-    // of angles, instead of a loop over them
+    // up to 512 tokens: a workgroup for every 256 lanes' heads, each with its own
+    // table of angles, instead of a loop over them (F16, 32 / 8 heads of 128: 4.5 ->
+    // 3.5 us for one token, 5.5 -> 4.6 for 256, 6.4 -> 6.2 for 512; 1024 10.9 -> 11.2)
     const int rows = (p.q != nullptr ? p.n_head : 0) + 2 * p.a.n_head_kv, pass = 2048 / p.a.head_dim;
-    const dim3 grid((unsigned)p.a.n_tok, p.a.n_tok < 128 ? (unsigned)((rows + pass - 1) / pass) : 1u), block(256);
+    const dim3 grid((unsigned)p.a.n_tok, p.a.n_tok <= 512 ? (unsigned)((rows + pass - 1) / pass) : 1u), block(256);
     if (p.a.head_dim == 128) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 128>), grid, block, 0, s, p);
     else if (p.a.head_dim == 64) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 64>), grid, block, 0, s, p);
     else if constexpr (KVT != SFA_KV_Q8_0) hipLaunchKernelGGL((norm_rope_append_kernel<KVT, 32>), grid, block, 0, s, p);

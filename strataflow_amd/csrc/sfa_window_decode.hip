@@ -7,13 +7,13 @@
 // K is under way from the end of the first product on and the next V from the
 // end of the second, so that one buffer each does and LDS has room for twice
 // the waves that two would leave (Q8_0, 8 sequences, window 8192, with append
-// and merge: 49 -> 47 us; one F16 token 12.2 -> 12.0).  The waves of a
+// and merge: 48.0 -> 45.5 us; one F16 token 11.9 -> 11.5).  The waves of a
 // workgroup, then the workgroups of a sequence (the merge kernel), join their
 // (maximum, sum, output).
 //
 // Measured (32 / 8 heads of 128): F16, 64 sequences, window 4096: 185 us, 5.8
-// TB/s.  Q8_0, 8 sequences, window 8192: 37 us of kernel, 3.9 TB/s; its loads
-// alone take 33 (rows of 136 bytes), its arithmetic alone 28.
+// TB/s.  Q8_0, 8 sequences, window 8192: 34.6 us of kernel, 4.0 TB/s; its loads
+// alone take 30 (rows of 136 bytes), its arithmetic alone 26.
 //
 // S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions: their 16 columns
 // are the G query heads of a kv head, and lane l holds column l % 16 of both,

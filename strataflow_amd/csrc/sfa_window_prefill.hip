@@ -13,6 +13,14 @@
 //
 // Chunks of few rows leave CUs idle: their tiles are split over workgroups,
 // whose records window_merge_kernel joins.
+//
+// Measured (32 / 8 heads of 128): F16, 4096 tokens on 8192, window 4096: 508 us,
+// 541 TFLOP/s of what the tokens see, which is 1083 on the matrix cores (a large
+// f16 product of the library: 1073; the clock falls to 1.7 GHz to 2 GHz under
+// either).  Q8_0, 777 tokens on 6000, window 1024: 71 us; F32 (16 / 4 heads),
+// 1500 tokens, window 512: 47 us: bound by the chain of a tile (its values into
+// halves, a barrier, products, a barrier) on two workgroups a CU, matrix cores
+// busy 21 % and 15 %.
 #include <type_traits>
 
 #include "sfa_window_dev.h"
