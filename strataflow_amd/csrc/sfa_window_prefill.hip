@@ -430,16 +430,17 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
     half8 qh[KC], ql[KC];
     const float f = score_factor(p.scale_log2, split_q<HD>(p.q + ((int64_t)b.tok * p.n_head + b.head) * HD + 8 * hh, qh, ql));
 
-    // What a thread brings of a tile.  F32: 1/8 of a row of K and of V.  Q8_0: a
-    // block; with HD 128 one of K and one of V, with HD 64 the first two waves
-    // have K's and the others V's.
+    // What a thread brings of a tile.  F32: 1/8 of a row of K and of V, four
+    // neighbouring values of every 32, so that a load instruction reads whole
+    // lines.  Q8_0: a block; with HD 128 one of K and one of V, with HD 64 the
+    // first two waves have K's and the others V's.
     const int col_bytes = p.n_head_kv * T::RB;
     constexpr int FPT = HD / 8;
     constexpr int UN = kQ8 ? NB / 2 : 2, WORDS = kQ8 ? 9 : FPT;
     const int unit = kQ8 && NB == 2 ? threadIdx.x & 127 : threadIdx.x;
     const int u_row = kQ8 ? unit / NB : unit / 8, u_blk = kQ8 ? unit % NB : unit % 8;
     // (a block's nine words start at its first multiple of 4)
-    const int u_off = u_row * col_bytes + (kQ8 ? kQ8Bytes * u_blk - 2 * (u_blk & 1) : 4 * FPT * u_blk);
+    const int u_off = u_row * col_bytes + (kQ8 ? kQ8Bytes * u_blk - 2 * (u_blk & 1) : 16 * u_blk);
     uint32_t raw[UN][WORDS];
     auto issue = [&](int t) {
         const Src s = source<TP, T::RB>(p, b, pages, t, lane);
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
             const auto r = buffer_of((UN == 2 ? u == 0 : wave < 2) ? s.k : s.v, s.bytes);
 #pragma unroll
             for (int i = 0; i + 4 <= WORDS; i += 4) {
-                const intx4 x = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(r, u_off - s.back, 4 * i, 0));
+                const intx4 x = __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(r, u_off - s.back, (kQ8 ? 4 : 32) * i, 0));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) raw[u][i + j] = x[j];
             }
@@ -502,22 +503,16 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
         }
     };
     auto stage_f32 = [&]() {
-        // 1/8 of a row as halves: 2 FPT bytes, chunks of 16 (HD 32: half a chunk)
         auto put = [&](const float (&x)[FPT], uint8_t *hi, uint8_t *lo, bool v) {
 #pragma unroll
-            for (int i = 0; i < FPT; i += FPT < 8 ? 4 : 8) {
-                half2v h[4], r[4];
-#pragma unroll
-                for (int j = 0; j < (FPT < 8 ? 2 : 4); ++j) split2_f16(x[i + 2 * j], x[i + 2 * j + 1], h[j], r[j]);
-                const int e = FPT * u_blk + i, ch = e / 8, in = e % 8 * 2;
-                const int at = u_row * T::ROW + 16 * (v ? pv_slot<HD>(u_row, ch) : pk_slot<HD>(u_row, ch)) + in;
-                if constexpr (FPT < 8) {
-                    *reinterpret_cast<half4 *>(hi + at) = half4{h[0][0], h[0][1], h[1][0], h[1][1]};
-                    *reinterpret_cast<half4 *>(lo + at) = half4{r[0][0], r[0][1], r[1][0], r[1][1]};
-                } else {
-                    *reinterpret_cast<half8 *>(hi + at) = half8{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
-                    *reinterpret_cast<half8 *>(lo + at) = half8{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
-                }
+            for (int i = 0; i < FPT; i += 4) {
+                half2v h0, h1, r0, r1;
+                split2_f16(x[i], x[i + 1], h0, r0);
+                split2_f16(x[i + 2], x[i + 3], h1, r1);
+                const int ch = i + u_blk / 2;
+                const int at = u_row * T::ROW + 16 * (v ? pv_slot<HD>(u_row, ch) : pk_slot<HD>(u_row, ch)) + 8 * (u_blk & 1);
+                *reinterpret_cast<half4 *>(hi + at) = half4{h0[0], h0[1], h1[0], h1[1]};
+                *reinterpret_cast<half4 *>(lo + at) = half4{r0[0], r0[1], r1[0], r1[1]};
             }
         };
         float x[FPT], amax = 0.0f, down, up;
@@ -703,8 +698,8 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
         } else {
             if (any_bad(v_bad))
                 bad |= spoiled<HD>(p, src, b.tpos, hh, [&](int r, int e) {
-                    const int th = r * 8 + e / FPT;
-                    return (v_bad[th / 64] >> th % 64 & 1) & (v_bits[th] >> e % FPT & 1);
+                    const int th = r * 8 + e % 32 / 4;
+                    return (v_bad[th / 64] >> th % 64 & 1) & (v_bits[th] >> (e / 32 * 4 + e % 4) & 1);
                 });
         }
     }
