@@ -150,10 +150,26 @@ __device__ inline void page_window(const WindowParams &p, const Block &b, PageWi
         pages.load(p.page_table, p.max_pages, page_of(p, (t < b.sink_tiles ? t : b.lo / TP + t - b.sink_tiles) * TP), lane);
 }
 
-// Whether the token at tpos sees row r of a tile.
-__device__ inline bool sees(const WindowParams &p, const Src &s, int r, int tpos) {
-    const int pos = s.first + r;
-    return (r >= s.from) & (r < s.to) & (pos <= tpos) & (s.sink | (pos > tpos - p.window) | (pos < p.n_sink)) & s.there;
+// The rows of a tile that the token at tpos sees, a bit each.
+__device__ inline uint64_t seen_rows(const WindowParams &p, const Src &s, int tpos) {
+    auto below = [](int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; };
+    const int at = tpos - s.first;
+    uint64_t m = below(min(s.to, at + 1)) & ~below(s.from);
+    if (!s.sink) m &= ~below(max(at, 0) + 1 - p.window) | below(p.n_sink - s.first);
+    return m;
+}
+
+// Scores [32 x][16], rows 32 x + 8 (i / 4) + 4 hh + i % 4, of the rows that are
+// not seen become -inf: three instructions a score (by comparisons of positions: 15).
+template <int PB>
+__device__ inline void mask_scores(const WindowParams &p, const Src &src, int tpos, int hh, floatx16 (&s)[PB]) {
+    asm("" : "+v"(tpos), "+v"(hh));  // (nothing of them held over the loop)
+    const uint64_t m = seen_rows(p, src, tpos) >> (4 * hh);
+#pragma unroll
+    for (int i = 0; i < 16 * PB; ++i) {
+        const uint32_t word = (uint32_t)(i < 16 ? m : m >> 32);
+        s[i / 16][i % 16] = word >> (i / 4 % 4 * 8 + i % 4) & 1 ? s[i / 16][i % 16] : -INFINITY;
+    }
 }
 
 // A value of V that is not finite would reach rows that do not see it, as 0
@@ -190,9 +206,11 @@ __device__ inline bool any_bad(const uint64_t *bad) { return __ballot((bad[0] | 
 // that leaves o alone: it hardly ever runs, and the registers are full.
 template <int HD, typename Was>
 __device__ inline uint64_t spoiled(const WindowParams &p, const Src &s, int tpos, int hh, Was was) {
+    asm("" : "+v"(tpos));  // (nothing of it held over the tile's products)
     uint64_t bits = 0;
+    const uint64_t seen = seen_rows(p, s, tpos);
     for (int r = s.from; r < s.to; ++r) {
-        if (!sees(p, s, r, tpos)) continue;
+        if ((seen >> r & 1) == 0) continue;
 #pragma unroll 1
         for (int j = 0; j < HD / 2; ++j)
             bits |= (uint64_t)was(r, j / 16 * 32 + j % 16 / 4 * 8 + 4 * hh + j % 4) << j;
@@ -331,13 +349,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_f16_kernel(WindowParams
                 s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[c], s[x], 0, 0, 0);
                 s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[c], s[x], 0, 0, 0);
             });
-        if (src.masked) {
-            int h4 = 4 * hh;
-            asm("" : "+v"(h4));  // (not 32 row numbers held over the loop)
-#pragma unroll
-            for (int i = 0; i < 16 * PB; ++i)
-                s[i / 16][i % 16] = sees(p, src, i / 16 * 32 + i / 4 % 4 * 8 + h4 + i % 4, b.tpos) ? s[i / 16][i % 16] : -INFINITY;
-        }
+        if (src.masked) mask_scores<PB>(p, src, b.tpos, hh, s);
         float mx = -INFINITY, x, y;
 #pragma unroll
         for (int i = 0; i < 16 * PB; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
@@ -626,13 +638,7 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
                     }
                 });
         }
-        if (src.masked) {
-            int h4 = 4 * hh;
-            asm("" : "+v"(h4));  // (not 32 row numbers held over the loop)
-#pragma unroll
-            for (int i = 0; i < 16 * PB; ++i)
-                s[i / 16][i % 16] = sees(p, src, i / 16 * 32 + i / 4 % 4 * 8 + h4 + i % 4, b.tpos) ? s[i / 16][i % 16] : -INFINITY;
-        }
+        if (src.masked) mask_scores<PB>(p, src, b.tpos, hh, s);
         float mx = -INFINITY, ma, mb;
 #pragma unroll
         for (int x = 0; x < PB; ++x)
