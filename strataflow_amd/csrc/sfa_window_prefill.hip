@@ -14,10 +14,10 @@
 // Chunks of few rows leave CUs idle: their tiles are split over workgroups,
 // whose records window_merge_kernel joins.
 //
-// Measured (32 / 8 heads of 128): F16, 4096 tokens on 8192, window 4096: 508 us,
-// 541 TFLOP/s of what the tokens see, which is 1083 on the matrix cores (a large
+// Measured (32 / 8 heads of 128): F16, 4096 tokens on 8192, window 4096: 503 us,
+// 547 TFLOP/s of what the tokens see, which is 1095 on the matrix cores (a large
 // f16 product of the library: 1073; the clock falls to 1.7 GHz to 2 GHz under
-// either).  Q8_0, 777 tokens on 6000, window 1024: 71 us; F32 (16 / 4 heads),
+// either).  Q8_0, 777 tokens on 6000, window 1024: 68 us; F32 (16 / 4 heads),
 // 1500 tokens, window 512: 47 us: bound by the chain of a tile (its values into
 // halves, a barrier, products, a barrier) on two workgroups a CU, matrix cores
 // busy 21 % and 15 %.
@@ -716,9 +716,9 @@ __global__ __launch_bounds__(256, 2) void window_prefill_wide_kernel(WindowParam
 // time.  A tile takes `tile` us where a CU has one workgroup, `pair` times that
 // where two share it (and in proportion beyond); every split writes and reads
 // its rows' records, at 3.5 TB/s.  Measured (us; 32 / 8 heads of 128): F16 93
-// tokens on 20100, window 4096: 164 / 54 / 37 / 39 with 1 / 4 / 10 / 21; Q8_0
-// 777 on 6000, window 1024: 98 / 83 / 94 with 1 / 2 / 3; F32 (16 / 4 heads) 1500
-// tokens, window 512: 64 / 59 / 67 with 1 / 2 / 4.
+// tokens on 20100, window 4096: 146 / 50 / 36 / 35 with 1 / 4 / 10 / 21; Q8_0
+// 777 on 6000, window 1024: 90 / 78 / 87 with 1 / 2 / 3; F32 (16 / 4 heads) 1500
+// tokens, window 512: 54 / 51 / 56 with 1 / 2 / 4.
 int window_prefill_splits(const sfa_kv_desc *kv, int32_t q_pos0, int32_t T, int32_t window, int32_t n_sink) {
     const bool f32 = kv->kv_type == SFA_KV_F32, f16 = kv->kv_type == SFA_KV_F16;
     const int tp = f32 ? 32 : 64, g = kv->n_head / kv->n_head_kv;
